@@ -14,8 +14,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 OBJ = os.path.join(HERE, 'csrc', '_obj')
 LIB = os.path.join(HERE, 'libavcap_hip.so')
-SOURCES = ['fused_mlp.hip', 'conv_enc.hip', 'misc.hip', 'mesh.hip', 'raster.hip', 'fusion.hip', 'knn_lbs.hip', 'render.hip', 'pack.cpp', 'capi.cpp']
-HEADERS = ['avcap_internal.h', 'mlp_layout.h', 'mc_tables.h', 'store_settle.h', os.path.join('..', '..', 'include', 'avcap.h')]
+SOURCES = ['fused_mlp.hip', 'conv_enc.hip', 'misc.hip', 'mesh.hip', 'raster.hip', 'fusion.hip', 'knn_lbs.hip', 'render.hip', 'linear.hip', 'layer_norm.hip', 'pack.cpp', 'capi.cpp']
+HEADERS = ['avcap_internal.h', 'linear.h', 'mlp_layout.h', 'mc_tables.h', 'store_settle.h', os.path.join('..', '..', 'include', 'avcap.h')]
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-Wno-unused-value', '-Wno-unused-result']
 # gfx950 / ROCm 7.2: a VGPR written by a packed-f32 VALU instruction and read as the data of a multi-dword store an instruction later reached memory stale in
@@ -26,7 +26,7 @@ NOPK = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 # mesh / KNN kernels promise bit-exact agreement with the C oracle (built with -ffp-contract=off):
 # HIP's __fmul_rn/__fadd_rn are plain operators, so contraction has to be disabled per file.
 EXTRA = {'mesh.hip': ['-ffp-contract=off'] + NOPK, 'knn_lbs.hip': ['-ffp-contract=off'] + NOPK, 'raster.hip': ['-ffp-contract=off'] + NOPK, 'render.hip': ['-ffp-contract=off'] + NOPK,
-         'misc.hip': NOPK, 'fusion.hip': NOPK,
+         'misc.hip': NOPK, 'fusion.hip': NOPK, 'linear.hip': NOPK, 'layer_norm.hip': NOPK, 'linear_tile.hip': NOPK,
          # MFMA accumulators in VGPRs: the epilogue reads them without a v_accvgpr_read per value (-0.7 % launch time, tools/ablate_run.sh)
          # (fused_mlp.hip without packed f32 as well: hipcc's SLP-packed v_pk_*_f32 cost issue time beside the MFMAs -- same-box A/B of the dense launch -1.0 % shader cycles)
          # -amdgpu-sched-strategy=max-ilp: what the scheduler does with the code between the pinned pieces; same bits, -1.1 % shader cycles per dense launch (tools/ab_flags.sh;
@@ -59,6 +59,8 @@ def build(force: bool = False, verbose: bool = True, asan: bool = False) -> str:
     # and a third time with the Softplus layers' weight scale undone in the epilogue (-DAVC_LAYER_SCALE=1: namespace `scaled`, pack.cpp add_warp)
     units = [(src + '.o', src, []) for src in SOURCES] + [('fused_mlp_checked.o', 'fused_mlp.hip', ['-DAVC_CHECK_RANGE=1']),
                                                           ('fused_mlp_scaled.o', 'fused_mlp.hip', ['-DAVC_LAYER_SCALE=1'])]
+    # the dense layer's tiled products, once per element type
+    units += [(f'linear_tile_{t}.o', 'linear_tile.hip', [f'-DAVC_LIN_{t.upper()}=1']) for t in ('f32', 'bf16', 'f16')]
     for obj, src, extra in units:
         sp = os.path.join(CSRC, src)
         op = os.path.join(OBJ, obj)

@@ -4,6 +4,7 @@
 #include <algorithm>
 
 #include "avcap_internal.h"
+#include "linear.h"
 
 namespace avc {
 const char *last_error();
@@ -291,6 +292,129 @@ int avc_group_norm(avc_ctx *ctx, const float *x, int N, int C, int64_t HW, int G
     AVC_REQUIRE((int64_t)N * C <= 1 << 30, AVC_ERR_ARG, "avc_group_norm: N * C too large");
     AVC_HIP(hipSetDevice(ctx->device));
     return launch_group_norm(ctx, x, N, C, HW, G, gamma, beta, eps, relu, y, (hipStream_t)stream);
+}
+
+// ---- dense layer, layer norm --------------------------------------------------------------------------------------------------------------------
+static int check_linear(const char *who, int64_t M, int64_t N, int64_t K, int dtype)
+{
+    constexpr int64_t TOP = (int64_t)1 << 31;
+    AVC_REQUIRE(dtype >= AVC_F32 && dtype <= AVC_F16, AVC_ERR_ARG, "%s: unknown dtype %d", who, dtype);
+    AVC_REQUIRE(M >= 0 && N >= 1 && K >= 1 && M < TOP && N < TOP && K < TOP, AVC_ERR_ARG, "%s: need 0 <= M, 1 <= N, 1 <= K, all below 2^31 (got %lld, %lld, %lld)", who, (long long)M,
+                (long long)N, (long long)K);
+    return AVC_OK;
+}
+static int check_x(const char *who, int64_t x_row, int64_t x_col, int64_t M, int64_t K)
+{
+    constexpr int64_t TOP = (int64_t)1 << 40;
+    AVC_REQUIRE((x_col == 1 || x_row == 1) && x_row >= 0 && x_col >= 0 && x_row < TOP && x_col < TOP, AVC_ERR_ARG, "%s: one of x's strides has to be 1 and none negative (got %lld, %lld)", who,
+                (long long)x_row, (long long)x_col);
+    return AVC_OK;
+}
+static avc::lin::Operand x_operand(const void *x, int64_t x_row, int64_t x_col) { return x_col == 1 ? avc::lin::Operand{x, x_row, 1} : avc::lin::Operand{x, x_col, 0}; }
+
+// The calls below run on the context's device and leave the thread's current device as they found it.
+struct DeviceGuard {
+    int was = -1;
+    bool ok;
+    explicit DeviceGuard(int device)
+    {
+        ok = hipGetDevice(&was) == hipSuccess;
+        if (ok && was != device) ok = hipSetDevice(device) == hipSuccess;
+        else was = -1;
+    }
+    ~DeviceGuard() { if (was >= 0) hipSetDevice(was); }
+};
+#define AVC_ON_DEVICE(ctx)                                                                                       \
+    DeviceGuard guard_((ctx)->device);                                                                           \
+    AVC_REQUIRE(guard_.ok, AVC_ERR_HIP, "cannot make device %d current", (ctx)->device)
+
+int avc_linear_workspace(int64_t M, int64_t N, int64_t K, int dtype, int64_t x_row, int64_t x_col, int64_t *bytes)
+{
+    AVC_REQUIRE(bytes, AVC_ERR_ARG, "avc_linear_workspace: NULL argument");
+    if (int rc = check_linear("avc_linear_workspace", M, N, K, dtype)) return rc;
+    if (int rc = check_x("avc_linear_workspace", x_row, x_col, M, K)) return rc;
+    *bytes = (int64_t)lin::forward_workspace(M, N, K, dtype, x_col == 1);
+    return AVC_OK;
+}
+
+int avc_linear(avc_ctx *ctx, const void *x, int64_t x_row, int64_t x_col, const void *w, int64_t ldw, const void *bias, const void *res, int64_t ldr, int act, float slope, int64_t M, int64_t N,
+               int64_t K, int dtype, void *y, int64_t ldy, void *z, int64_t ldz, void *workspace, int64_t workspace_bytes, avc_stream stream)
+{
+    if (int rc = check_linear("avc_linear", M, N, K, dtype)) return rc;
+    AVC_REQUIRE(ctx && (!M || (x && w && y)), AVC_ERR_ARG, "avc_linear: NULL argument");
+    if (int rc = check_x("avc_linear", x_row, x_col, M, K)) return rc;
+    AVC_REQUIRE(act >= AVC_ACT_NONE && act <= AVC_ACT_SILU, AVC_ERR_ARG, "avc_linear: unknown activation %d", act);
+    AVC_REQUIRE(ldw >= 0 && ldy >= N && (!res || ldr >= 0) && (!z || ldz >= N), AVC_ERR_ARG, "avc_linear: a row stride is negative, or an output's shorter than its row");
+    AVC_REQUIRE(((uintptr_t)workspace & 15) == 0 && workspace_bytes >= (int64_t)lin::forward_workspace(M, N, K, dtype, x_col == 1) && (workspace || !workspace_bytes), AVC_ERR_CAPACITY,
+                "avc_linear: needs %lld bytes of 16-byte aligned workspace, got %lld", (long long)lin::forward_workspace(M, N, K, dtype, x_col == 1), (long long)workspace_bytes);
+    if (!M) return AVC_OK;
+    AVC_ON_DEVICE(ctx);
+    const lin::Epilogue e{bias, res, res ? ldr : 0, z, z ? ldz : 0, act, slope};
+    return lin::forward(x_operand(x, x_row, x_col), w, ldw, M, N, K, dtype, e, y, ldy, workspace, (hipStream_t)stream);
+}
+
+int avc_linear_backward_workspace(int64_t M, int64_t N, int64_t K, int dtype, int64_t *bytes)
+{
+    AVC_REQUIRE(bytes, AVC_ERR_ARG, "avc_linear_backward_workspace: NULL argument");
+    if (int rc = check_linear("avc_linear_backward_workspace", M, N, K, dtype)) return rc;
+    *bytes = (int64_t)lin::backward_workspace(M, N, K, dtype);
+    return AVC_OK;
+}
+
+int avc_linear_backward(avc_ctx *ctx, const void *dy, int64_t lddy, const void *x, int64_t x_row, int64_t x_col, const void *w, int64_t ldw, const void *saved, int64_t ld_saved, int act,
+                        float slope, int64_t M, int64_t N, int64_t K, int dtype, void *dx, void *dw, void *db, void *workspace, int64_t workspace_bytes, avc_stream stream)
+{
+    if (int rc = check_linear("avc_linear_backward", M, N, K, dtype)) return rc;
+    AVC_REQUIRE(act >= AVC_ACT_NONE && act <= AVC_ACT_SILU, AVC_ERR_ARG, "avc_linear_backward: unknown activation %d", act);
+    AVC_REQUIRE(ctx && (!M || (dy && (!dw || x) && (!dx || w) && (act == AVC_ACT_NONE || saved))), AVC_ERR_ARG, "avc_linear_backward: NULL argument");
+    if (dw)
+        if (int rc = check_x("avc_linear_backward", x_row, x_col, M, K)) return rc;
+    AVC_REQUIRE(lddy >= 0 && ldw >= 0 && (act == AVC_ACT_NONE || ld_saved >= 0), AVC_ERR_ARG, "avc_linear_backward: a row stride is negative");
+    AVC_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= (int64_t)lin::backward_workspace(M, N, K, dtype), AVC_ERR_CAPACITY,
+                "avc_linear_backward: needs %lld bytes of 16-byte aligned workspace, got %lld", (long long)lin::backward_workspace(M, N, K, dtype), (long long)workspace_bytes);
+    AVC_ON_DEVICE(ctx);
+    return lin::backward(dy, lddy, x_operand(x, x_row, x_col), w, ldw, saved, ld_saved, act, slope, M, N, K, dtype, dx, dw, db, workspace, (hipStream_t)stream);
+}
+
+static int check_norm(const char *who, int64_t M, int64_t C, int dtype)
+{
+    constexpr int64_t TOP = (int64_t)1 << 31;
+    AVC_REQUIRE(dtype >= AVC_F32 && dtype <= AVC_F16, AVC_ERR_ARG, "%s: unknown dtype %d", who, dtype);
+    AVC_REQUIRE(M >= 0 && C >= 1 && M < TOP && C < TOP, AVC_ERR_ARG, "%s: need 0 <= M, 1 <= C, both below 2^31 (got %lld, %lld)", who, (long long)M, (long long)C);
+    return AVC_OK;
+}
+
+int avc_layer_norm(avc_ctx *ctx, const void *x, int64_t ldx, const void *gamma, const void *beta, float eps, int64_t M, int64_t C, int dtype, void *y, int64_t ldy, float *mean, float *rstd,
+                   avc_stream stream)
+{
+    if (int rc = check_norm("avc_layer_norm", M, C, dtype)) return rc;
+    AVC_REQUIRE(ctx && (!M || (x && y)) && !mean == !rstd, AVC_ERR_ARG, "avc_layer_norm: NULL argument, or one of mean and rstd without the other");
+    AVC_REQUIRE(ldx >= 0 && ldy >= C, AVC_ERR_ARG, "avc_layer_norm: ldx is negative or ldy shorter than the row");
+    AVC_REQUIRE(eps >= 0.f, AVC_ERR_ARG, "avc_layer_norm: eps must be >= 0 (got %g)", (double)eps);
+    if (!M) return AVC_OK;
+    AVC_ON_DEVICE(ctx);
+    return lin::layer_norm(x, ldx, gamma, beta, eps, M, C, dtype, y, ldy, mean, rstd, (hipStream_t)stream);
+}
+
+int avc_layer_norm_backward_workspace(int64_t M, int64_t C, int dtype, int64_t *bytes)
+{
+    AVC_REQUIRE(bytes, AVC_ERR_ARG, "avc_layer_norm_backward_workspace: NULL argument");
+    if (int rc = check_norm("avc_layer_norm_backward_workspace", M, C, dtype)) return rc;
+    *bytes = (int64_t)lin::layer_norm_backward_workspace(M, C, dtype);
+    return AVC_OK;
+}
+
+int avc_layer_norm_backward(avc_ctx *ctx, const void *dy, int64_t lddy, const void *x, int64_t ldx, const void *gamma, const float *mean, const float *rstd, int64_t M, int64_t C, int dtype,
+                            void *dx, int64_t lddx, void *dgamma, void *dbeta, void *workspace, int64_t workspace_bytes, avc_stream stream)
+{
+    if (int rc = check_norm("avc_layer_norm_backward", M, C, dtype)) return rc;
+    AVC_REQUIRE(ctx && (!M || (dy && x && mean && rstd)), AVC_ERR_ARG, "avc_layer_norm_backward: NULL argument");
+    AVC_REQUIRE(ldx >= 0 && lddy >= 0 && (!dx || lddx >= C), AVC_ERR_ARG, "avc_layer_norm_backward: a row stride is negative or lddx shorter than the row");
+    if (dgamma || dbeta)
+        AVC_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= (int64_t)lin::layer_norm_backward_workspace(M, C, dtype), AVC_ERR_CAPACITY,
+                    "avc_layer_norm_backward: needs %lld bytes of 16-byte aligned workspace, got %lld", (long long)lin::layer_norm_backward_workspace(M, C, dtype), (long long)workspace_bytes);
+    AVC_ON_DEVICE(ctx);
+    return lin::layer_norm_backward(dy, lddy, x, ldx, gamma, mean, rstd, M, C, dtype, dx, lddx, dgamma, dbeta, (float *)workspace, (hipStream_t)stream);
 }
 
 int avc_scatter_volume(avc_ctx *ctx, const uint8_t *valid, int64_t N, const float *values, const float *fill, float *vol, avc_stream stream)

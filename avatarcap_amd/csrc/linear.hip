@@ -1,0 +1,415 @@
+// The dense layer y = act(x W^T + b) + r and its gradients (include/avcap.h avc_linear, avc_linear_backward): which kernel serves which sizes, and the kernels around the
+// tiled product (linear_tile.hip): few rows, few columns of channel-first points, sums of the splits, the activation's gradient with the bias gradient.
+#include <algorithm>
+#include "avcap_internal.h"
+#include "linear.h"
+
+namespace avc { namespace lin {
+
+namespace {
+
+// ---- one stored value with the epilogue applied ---------------------------------------------------------------------------------------------------------------
+template <typename T> __device__ __forceinline__ void finish(float v, int64_t m, int64_t n, const Epilogue &e, T *out, int64_t ldo)
+{
+    if (e.bias) v += (float)((const T *)e.bias)[n];
+    if (e.z) ((T *)e.z)[m * e.ldz + n] = (T)v;
+    float a[1] = {v};
+    act_run<1>(a, e.act, e.slope);
+    v = a[0];
+    if (e.res) v += (float)((const T *)e.res)[m * e.ldr + n];
+    out[m * ldo + n] = (T)v;
+}
+
+// ---- sums of the splits: one thread per output value, the splits added in order ----------------------------------------------------------------------------------
+template <typename T> __global__ __launch_bounds__(256) void reduce_kernel(const float *__restrict__ part, int splits, int64_t M, int64_t N, T *out, int64_t ldo, const Epilogue e)
+{
+    const int64_t total = M * N;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        float v = 0.f;
+        for (int s = 0; s < splits; ++s) v += part[s * total + i];
+        finish<T>(v, i / N, i % N, e, out, ldo);
+    }
+}
+
+// ---- few rows: out(f, s) = sum_k F(f, k) S(s, k) with at most 16 * FB rows f against a long operand S that is read once -------------------------------------------
+// A wave takes 16 rows of S and all rows of F on 16-row matrix instructions; the k axis is dealt in chunks of 128 bytes per row to the workgroup's waves, whose sums meet in
+// LDS.  Lane (row l, quarter q) loads 32 adjacent bytes of its row, so a row's chunk is one 128-byte line.  float32 uses the f32 matrix instruction: the call is bound by the
+// read of S, not by products.
+template <typename T> struct FewArgs { const T *S; int64_t lds; const T *F; int64_t ldf; int64_t ns; int nf; int64_t K; int rows_are_f; Epilogue ep; T *out; int64_t ldo; int kw; };
+
+template <typename T> struct Chunk { static constexpr int LANE = 32 / sizeof(T), K = 4 * LANE; typedef T vec __attribute__((ext_vector_type(LANE))); vec v; };
+
+template <typename T> __device__ __forceinline__ Chunk<T> load_chunk(const T *row, int64_t k, int64_t K)
+{
+    Chunk<T> c;
+    if (k + Chunk<T>::LANE <= K) __builtin_memcpy(&c.v, row + k, sizeof c.v);
+    else
+#pragma unroll
+        for (int j = 0; j < Chunk<T>::LANE; ++j) c.v[j] = k + j < K ? row[k + j] : (T)0.f;
+    return c;
+}
+
+__device__ __forceinline__ f32x4 chunk_mfma(const Chunk<float> &a, const Chunk<float> &b, f32x4 c)
+{
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[j], b.v[j], c, 0, 0, 0);
+    return c;
+}
+__device__ __forceinline__ f32x4 chunk_mfma(const Chunk<__bf16> &a, const Chunk<__bf16> &b, f32x4 c)
+{
+    typedef bf16x8 h;
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(h(a.v.lo), h(b.v.lo), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(h(a.v.hi), h(b.v.hi), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 chunk_mfma(const Chunk<_Float16> &a, const Chunk<_Float16> &b, f32x4 c)
+{
+    typedef f16x8 h;
+    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(h(a.v.lo), h(b.v.lo), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(h(a.v.hi), h(b.v.hi), c, 0, 0, 0);
+}
+
+template <typename T, int FB> __global__ __launch_bounds__(1024) void few_kernel(const FewArgs<T> a)
+{
+    __shared__ f32x4 sums[16][FB][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, kslot = wave % a.kw, group = wave / a.kw, groups = (blockDim.x >> 6) / a.kw;
+    const int l16 = lane & 15, q = lane >> 4;
+    const int64_t s0 = ((int64_t)blockIdx.x * groups + group) * 16;
+    // rows past the end repeat the last one: their results are not stored
+    const T *srow = a.S + min(s0 + l16, a.ns - 1) * a.lds;
+    const T *frow[FB];
+#pragma unroll
+    for (int b = 0; b < FB; ++b) frow[b] = a.F + (int64_t)min(16 * b + l16, a.nf - 1) * a.ldf;
+    f32x4 acc[FB];
+#pragma unroll
+    for (int b = 0; b < FB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    constexpr int CK = Chunk<T>::K, U = 4;
+    const int64_t stride = (int64_t)a.kw * CK;
+    int64_t k = (int64_t)kslot * CK;
+    for (; k + (U - 1) * stride + CK <= a.K; k += U * stride) {
+        Chunk<T> s[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) s[u] = load_chunk(srow, k + u * stride + q * Chunk<T>::LANE, a.K);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int b = 0; b < FB; ++b) acc[b] = chunk_mfma(s[u], load_chunk(frow[b], k + u * stride + q * Chunk<T>::LANE, a.K), acc[b]);
+    }
+    for (; k < a.K; k += stride) {
+        const Chunk<T> s = load_chunk(srow, k + q * Chunk<T>::LANE, a.K);
+#pragma unroll
+        for (int b = 0; b < FB; ++b) acc[b] = chunk_mfma(s, load_chunk(frow[b], k + q * Chunk<T>::LANE, a.K), acc[b]);
+    }
+    if (a.kw > 1) {
+#pragma unroll
+        for (int b = 0; b < FB; ++b) sums[wave][b][lane] = acc[b];
+        __syncthreads();
+        if (kslot) return;
+#pragma unroll
+        for (int b = 0; b < FB; ++b)
+            for (int w = 1; w < a.kw; ++w) acc[b] += sums[wave + w][b][lane];
+    }
+#pragma unroll
+    for (int b = 0; b < FB; ++b) {
+        const int f = 16 * b + l16;
+        if (f >= a.nf) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t s = s0 + 4 * q + j;
+            if (s < a.ns) finish<T>(acc[b][j], a.rows_are_f ? f : s, a.rows_are_f ? s : f, a.ep, a.out, a.ldo);
+        }
+    }
+}
+
+// ---- few output columns of channel-first points: y(m, n) = act(sum_k x[k][m] w[n][k] + b) with the points contiguous, N <= NB -------------------------------------
+// Bound by the read of x: lanes take adjacent points, the workgroup's four waves a quarter of k each, the weights come through LDS.
+template <typename T, int NB> __global__ __launch_bounds__(256) void narrow_kernel(const T *__restrict__ x, int64_t ldx, const T *__restrict__ w, int64_t ldw, int64_t M, int N, int64_t K,
+                                                                                   const Epilogue e, T *out, int64_t ldo)
+{
+    constexpr int V = 4, KT = 256;                                       // points per lane, k per pass
+    __shared__ float wk[KT][NB];
+    __shared__ float part[3][64][V * NB + 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t m = ((int64_t)blockIdx.x * 64 + lane) * V;
+    const bool full = m + V <= M;
+    float acc[NB][V] = {};
+    for (int64_t kb = 0; kb < K; kb += KT) {
+        const int kt = (int)min((int64_t)KT, K - kb);
+        __syncthreads();
+        for (int i = threadIdx.x; i < NB * KT; i += 256) {
+            const int n = i / KT, k = i % KT;
+            wk[k][n] = n < N && k < kt ? (float)w[n * ldw + kb + k] : 0.f;
+        }
+        __syncthreads();
+        if (m < M) {
+#pragma unroll 8
+            for (int k = wave; k < kt; k += 4) {
+                const T *src = x + (kb + k) * ldx + m;
+                T v[V];
+                if (full) __builtin_memcpy(v, src, sizeof v);
+                else
+#pragma unroll
+                    for (int j = 0; j < V; ++j) v[j] = m + j < M ? src[j] : (T)0.f;
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) acc[n][j] = fmaf((float)v[j], wk[k][n], acc[n][j]);
+            }
+        }
+    }
+    if (wave) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int j = 0; j < V; ++j) part[wave - 1][lane][n * V + j] = acc[n][j];
+    }
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float v = (acc[n][j] + part[0][lane][n * V + j]) + (part[1][lane][n * V + j] + part[2][lane][n * V + j]);
+            if (n < N && m + j < M) finish<T>(v, m + j, n, e, out, ldo);
+        }
+}
+
+// ---- the activation's gradient dz = dy act'(z), and the column sums of dz in the same pass -------------------------------------------------------------------------
+// Lanes take V adjacent columns, `tx` lanes a row, 256 / tx rows at a time; every workgroup walks a strip of rows and leaves its column sums in part[strip][N] (float32, a
+// fixed order), which colsum_kernel adds.  dz is rounded to the element type: it is the operand of two matrix products in that type.
+template <typename T, int V> __global__ __launch_bounds__(256) void dact_kernel(const T *__restrict__ dy, int64_t lddy, const T *__restrict__ z, int64_t ldz, int act, float slope, int64_t M, int64_t N,
+                                                                               int64_t rows_per, int tx, T *__restrict__ dz, float *__restrict__ part)
+{
+    typedef T vec __attribute__((ext_vector_type(V)));
+    const int lx = threadIdx.x % tx, ly = threadIdx.x / tx, ty = 256 / tx;
+    const int64_t n = ((int64_t)blockIdx.y * tx + lx) * V, m1 = min(M, ((int64_t)blockIdx.x + 1) * rows_per);
+    float sum[V] = {};
+    if (n < N) {
+#pragma unroll 2
+        for (int64_t m = blockIdx.x * rows_per + ly; m < m1; m += ty) {
+            vec g = *reinterpret_cast<const vec *>(dy + m * lddy + n);
+            float v[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = (float)g[j];
+            if (z) {
+                const vec s = *reinterpret_cast<const vec *>(z + m * ldz + n);
+                vec o;
+                float zs[V], sl[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) zs[j] = (float)s[j];
+                slope_run<V>(zs, sl, act, slope);
+#pragma unroll
+                for (int j = 0; j < V; ++j) { v[j] *= sl[j]; o[j] = (T)v[j]; }
+                *reinterpret_cast<vec *>(dz + m * N + n) = o;
+            }
+#pragma unroll
+            for (int j = 0; j < V; ++j) sum[j] += v[j];
+        }
+    }
+    if (!part) return;
+    __shared__ float red[256][V + 1];
+#pragma unroll
+    for (int j = 0; j < V; ++j) red[threadIdx.x][j] = sum[j];
+    __syncthreads();
+    if (ly || n >= N) return;
+    for (int y = 1; y < ty; ++y)
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[j] += red[y * tx + lx][j];
+#pragma unroll
+    for (int j = 0; j < V; ++j) part[(int64_t)blockIdx.x * N + n + j] = sum[j];
+}
+
+}  // namespace
+
+// out(n) = sum over the strips of part[strip][n]: 32 columns and 8 runs of strips per workgroup, the runs' sums added in order.  Columns past N1 belong to the second output.
+template <typename T> __global__ __launch_bounds__(256) void colsum_kernel(const float *__restrict__ part, int strips, int64_t N, int64_t N1, T *out, T *out2)
+{
+    __shared__ float red[8][33];
+    const int lx = threadIdx.x & 31, ly = threadIdx.x >> 5;
+    const int64_t n = (int64_t)blockIdx.x * 32 + lx;
+    float s = 0.f;
+    if (n < N)
+        for (int i = ly; i < strips; i += 8) s += part[(int64_t)i * N + n];
+    red[ly][lx] = s;
+    __syncthreads();
+    if (ly || n >= N) return;
+    for (int y = 1; y < 8; ++y) s += red[y][lx];
+    if (n < N1) { if (out) out[n] = (T)s; }
+    else if (out2) out2[n - N1] = (T)s;
+}
+
+static int launch_columns(const float *part, int strips, int64_t N, int64_t N1, int dtype, void *out, void *out2, hipStream_t s)
+{
+    const dim3 grid((unsigned)((N + 31) / 32));
+    if (dtype == AVC_F32) hipLaunchKernelGGL(colsum_kernel<float>, grid, dim3(256), 0, s, part, strips, N, N1, (float *)out, (float *)out2);
+    else if (dtype == AVC_BF16) hipLaunchKernelGGL(colsum_kernel<__bf16>, grid, dim3(256), 0, s, part, strips, N, N1, (__bf16 *)out, (__bf16 *)out2);
+    else hipLaunchKernelGGL(colsum_kernel<_Float16>, grid, dim3(256), 0, s, part, strips, N, N1, (_Float16 *)out, (_Float16 *)out2);
+    AVC_HIP(hipGetLastError());
+    return AVC_OK;
+}
+int launch_colsum2(const float *part, int strips, int64_t C, int dtype, void *out, void *out2, hipStream_t s) { return launch_columns(part, strips, 2 * C, C, dtype, out, out2, s); }
+
+namespace {
+
+inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// ---- which tile, how many splits: from the sizes alone, so that the workspace can be asked for in advance -----------------------------------------------------------
+struct Plan { int tile, tiles_m, tiles_n, splits; int64_t kper; };
+
+Plan plan_tiles(int64_t M, int64_t N, int64_t K, int dtype)
+{
+    Plan p;
+    const int bk = tile_bk(dtype);
+    auto count = [&](int t) { return cdiv(M, tile_bm(dtype, t)) * cdiv(N, tile_bn(dtype, t)); };
+    p.tile = M <= 64 || N <= 64 ? TILE_SMALL : (count(TILE_BIG) >= 192 && K >= 512 && N > 128 ? TILE_BIG : TILE_MID);
+    if (p.tile == TILE_MID && count(TILE_MID) * std::min<int64_t>(16, cdiv(K, 4 * bk)) < 128) p.tile = TILE_SMALL;
+    const int64_t tiles = count(p.tile);
+    p.tiles_m = (int)cdiv(M, tile_bm(dtype, p.tile));
+    p.tiles_n = (int)cdiv(N, tile_bn(dtype, p.tile));
+    int64_t splits = 1;
+    if (tiles < 256) splits = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512 / tiles, 256), K / (4 * bk)));
+    p.kper = cdiv(cdiv(K, splits), bk) * bk;
+    if (p.kper < bk) p.kper = bk;
+    p.splits = (int)std::max<int64_t>(1, cdiv(K, p.kper));
+    return p;
+}
+size_t partial_bytes(const Plan &p, int64_t M, int64_t N) { return p.splits > 1 ? sizeof(float) * (size_t)p.splits * (size_t)M * (size_t)N : 0; }
+
+// strips of the activation-gradient pass: enough workgroups to fill the chip, at least 8 rows each
+int64_t strips_for(int64_t M, int64_t N) { return std::max<int64_t>(1, std::min<int64_t>(cdiv(M, 8), std::max<int64_t>(1, 2048 / cdiv(N, 1024)))); }
+
+inline size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
+inline int esize(int dtype) { return dtype == AVC_F32 ? 4 : 2; }
+
+template <typename T> int launch_reduce(const float *part, int splits, int64_t M, int64_t N, void *out, int64_t ldo, const Epilogue &e, hipStream_t s)
+{
+    const int64_t blocks = std::min<int64_t>(cdiv(M * N, 256), 4096);
+    hipLaunchKernelGGL(reduce_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, part, splits, M, N, (T *)out, ldo, e);
+    AVC_HIP(hipGetLastError());
+    return AVC_OK;
+}
+
+int product(const Operand &P, const Operand &Q, int64_t M, int64_t N, int64_t K, int dtype, const Epilogue &e, void *out, int64_t ldo, void *ws, hipStream_t s)
+{
+    const Plan p = plan_tiles(M, N, K, dtype);
+    AVC_REQUIRE((int64_t)p.tiles_m * p.tiles_n * p.splits < (1 << 22), AVC_ERR_ARG, "avc_linear: %lld x %lld outputs are more than one launch covers", (long long)M, (long long)N);
+    TileArgs a{P, Q, M, N, K, out, ldo, e, (float *)ws, p.kper, p.tiles_m, p.tiles_n, p.splits};
+    const int rc = dtype == AVC_F32 ? launch_tile_f32(a, p.tile, s) : dtype == AVC_BF16 ? launch_tile_bf16(a, p.tile, s) : launch_tile_f16(a, p.tile, s);
+    if (rc != AVC_OK || p.splits == 1) return rc;
+    if (dtype == AVC_F32) return launch_reduce<float>(a.partial, p.splits, M, N, out, ldo, e, s);
+    if (dtype == AVC_BF16) return launch_reduce<__bf16>(a.partial, p.splits, M, N, out, ldo, e, s);
+    return launch_reduce<_Float16>(a.partial, p.splits, M, N, out, ldo, e, s);
+}
+
+// ---- few rows ----------------------------------------------------------------------------------------------------------------------------------------------------
+constexpr int FEW = 32;
+template <typename T> int launch_few(const void *S, int64_t lds, int64_t ns, const void *F, int64_t ldf, int nf, int64_t K, int rows_are_f, const Epilogue &e, void *out, int64_t ldo, hipStream_t s)
+{
+    FewArgs<T> a{(const T *)S, lds, (const T *)F, ldf, ns, nf, K, rows_are_f, e, (T *)out, ldo, 1};
+    const int64_t groups = cdiv(ns, 16), chunks = cdiv(K, Chunk<T>::K);
+    // waves that share a group's k axis: as many as bring the launch to ~4096 waves, no more than there are chunks
+    while (a.kw < 16 && groups * a.kw < 4096 && a.kw * 2 <= chunks) a.kw *= 2;
+    const int waves = std::max(4, a.kw), per = waves / a.kw;
+    AVC_REQUIRE(cdiv(groups, per) <= (1 << 22), AVC_ERR_ARG, "avc_linear: %lld rows are more than one launch covers", (long long)ns);
+    const dim3 grid((unsigned)cdiv(groups, per)), block(64 * waves);
+    if (nf <= 16) hipLaunchKernelGGL((few_kernel<T, 1>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((few_kernel<T, 2>), grid, block, 0, s, a);
+    AVC_HIP(hipGetLastError());
+    return AVC_OK;
+}
+
+template <typename T> int launch_narrow(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t M, int N, int64_t K, const Epilogue &e, void *out, int64_t ldo, hipStream_t s)
+{
+    const dim3 grid((unsigned)cdiv(M, 256));
+    if (N == 1) hipLaunchKernelGGL((narrow_kernel<T, 1>), grid, dim3(256), 0, s, (const T *)x, ldx, (const T *)w, ldw, M, N, K, e, (T *)out, ldo);
+    else hipLaunchKernelGGL((narrow_kernel<T, 4>), grid, dim3(256), 0, s, (const T *)x, ldx, (const T *)w, ldw, M, N, K, e, (T *)out, ldo);
+    AVC_HIP(hipGetLastError());
+    return AVC_OK;
+}
+
+#define AVC_BY_TYPE(dtype, call)                                         \
+    ((dtype) == AVC_F32 ? call<float> : (dtype) == AVC_BF16 ? call<__bf16> : call<_Float16>)
+
+enum Route { ROUTE_TILE, ROUTE_FEW_ROWS, ROUTE_FEW_COLS, ROUTE_NARROW };
+Route route(int64_t M, int64_t N, bool x_kc)
+{
+    if (x_kc && M <= FEW) return ROUTE_FEW_ROWS;
+    if (x_kc && N <= 16) return ROUTE_FEW_COLS;
+    if (!x_kc && N <= 4) return ROUTE_NARROW;
+    return ROUTE_TILE;
+}
+
+template <typename T> int launch_dact(const void *dy, int64_t lddy, const void *z, int64_t ldz, int act, float slope, int64_t M, int64_t N, void *dz, float *part, int64_t strips, hipStream_t s)
+{
+    constexpr int V = 16 / sizeof(T);
+    const bool wide = N % V == 0 && lddy % V == 0 && ((uintptr_t)dy & 15) == 0 && (!z || (ldz % V == 0 && ((uintptr_t)z & 15) == 0));
+    const int v = wide ? V : 1;
+    int tx = 1;
+    while (tx < 256 && (int64_t)tx * v < N) tx *= 2;
+    const dim3 grid((unsigned)strips, (unsigned)cdiv(N, (int64_t)tx * v));
+    const int64_t rows = cdiv(M, strips);
+    if (wide) hipLaunchKernelGGL((dact_kernel<T, V>), grid, dim3(256), 0, s, (const T *)dy, lddy, (const T *)z, ldz, act, slope, M, N, rows, tx, (T *)dz, part);
+    else hipLaunchKernelGGL((dact_kernel<T, 1>), grid, dim3(256), 0, s, (const T *)dy, lddy, (const T *)z, ldz, act, slope, M, N, rows, tx, (T *)dz, part);
+    AVC_HIP(hipGetLastError());
+    return AVC_OK;
+}
+
+}  // namespace
+
+size_t forward_workspace(int64_t M, int64_t N, int64_t K, int dtype, bool x_kc)
+{
+    return M && route(M, N, x_kc) == ROUTE_TILE ? partial_bytes(plan_tiles(M, N, K, dtype), M, N) : 0;
+}
+
+struct BackwardSpace { size_t dz, strips, partial, total; };
+static BackwardSpace backward_space(int64_t M, int64_t N, int64_t K, int dtype)
+{
+    BackwardSpace w;
+    w.dz = align256((size_t)M * N * esize(dtype));
+    w.strips = align256(sizeof(float) * (size_t)strips_for(M, N) * N);
+    w.partial = partial_bytes(plan_tiles(N, K, M, dtype), N, K);
+    if (M) w.partial = std::max(w.partial, partial_bytes(plan_tiles(M, K, N, dtype), M, K));
+    w.total = w.dz + w.strips + w.partial;
+    return w;
+}
+size_t backward_workspace(int64_t M, int64_t N, int64_t K, int dtype) { return backward_space(M, N, K, dtype).total; }
+
+int forward(const Operand &x, const void *w, int64_t ldw, int64_t M, int64_t N, int64_t K, int dtype, const Epilogue &e, void *y, int64_t ldy, void *ws, hipStream_t s)
+{
+    switch (route(M, N, x.kc)) {
+    case ROUTE_FEW_ROWS: return AVC_BY_TYPE(dtype, launch_few)(w, ldw, N, x.p, x.ld, (int)M, K, 1, e, y, ldy, s);
+    case ROUTE_FEW_COLS: return AVC_BY_TYPE(dtype, launch_few)(x.p, x.ld, M, w, ldw, (int)N, K, 0, e, y, ldy, s);
+    case ROUTE_NARROW: return AVC_BY_TYPE(dtype, launch_narrow)(x.p, x.ld, w, ldw, M, (int)N, K, e, y, ldy, s);
+    default: return product(x, Operand{w, ldw, 1}, M, N, K, dtype, e, y, ldy, ws, s);
+    }
+}
+
+int backward(const void *dy, int64_t lddy, const Operand &x, const void *w, int64_t ldw, const void *z, int64_t ldz, int act, float slope, int64_t M, int64_t N, int64_t K, int dtype,
+             void *dx, void *dw, void *db, void *ws, hipStream_t s)
+{
+    const BackwardSpace sp = backward_space(M, N, K, dtype);
+    char *dz_buf = (char *)ws, *strips_buf = dz_buf + sp.dz, *part = strips_buf + sp.strips;
+    const bool active = act != AVC_ACT_NONE;
+    if (active || db) {
+        const int64_t strips = strips_for(M, N);
+        const int rc = AVC_BY_TYPE(dtype, launch_dact)(dy, lddy, active ? z : nullptr, ldz, act, slope, M, N, dz_buf, db ? (float *)strips_buf : nullptr, strips, s);
+        if (rc != AVC_OK) return rc;
+        if (db) {
+            const int rc2 = launch_columns((const float *)strips_buf, (int)strips, N, N, dtype, db, nullptr, s);
+            if (rc2 != AVC_OK) return rc2;
+        }
+    }
+    const void *dz = active ? dz_buf : dy;
+    const int64_t lddz = active ? N : lddy;
+    const Epilogue none{nullptr, nullptr, 0, nullptr, 0, AVC_ACT_NONE, 0.f};
+    if (dx && M) {
+        const int rc = product(Operand{dz, lddz, 1}, Operand{w, ldw, 0}, M, K, N, dtype, none, dx, K, part, s);
+        if (rc != AVC_OK) return rc;
+    }
+    if (dw) {
+        const int rc = product(Operand{dz, lddz, 0}, Operand{x.p, x.ld, x.kc ? 0 : 1}, N, K, M, dtype, none, dw, K, part, s);
+        if (rc != AVC_OK) return rc;
+    }
+    return AVC_OK;
+}
+
+}}  // namespace avc::lin

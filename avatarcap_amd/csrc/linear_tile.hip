@@ -1,0 +1,438 @@
+// The dense layer's products (include/avcap.h avc_linear): out(i, j) = sum_k P(i, k) Q(j, k), either operand with k or its rows contiguous, bias / activation / residual in
+// the epilogue.  Built once per element type (-DAVC_LIN_F32 / _BF16 / _F16).
+//
+//   forward        y  = x W^T      P = x  (k contiguous, or the points when x is channel-first)   Q = W   (k contiguous)
+//   input gradient dx = dz W       P = dz (k contiguous)                                          Q = W   (rows contiguous)
+//   weight gradient dW = dz^T x    P = dz (rows contiguous)                                       Q = x   (rows contiguous, or k when x is channel-first)
+//
+// One workgroup computes a BM x BN tile; every wave a (BM / WM) x (BN / WN) part of it in v_mfma_f32_16x16x32 accumulators.  Q's rows are the matrix instruction's rows, so a
+// lane holds runs of 4 adjacent columns of one output row.  The epilogue passes them through the wave's own part of LDS, two fragment rows at a time: lanes then take 16 bytes of
+// a row each, adjacent lanes adjacent pieces, and one copy of the activation code serves all of the tile.
+//
+// float32 runs on the same bf16 matrix instructions: x = h + m + l, three bf16 of 8 significant bits each (rounded to nearest, so the three hold all 24 bits exactly), and
+// x w = hh + (hm + mh) + (hl + mm + lh) + terms below 2^-23 |x w| that float32's own products would round away.  Six products at the bf16 rate are faster than one at the f32
+// matrix rate.  The head is clamped to bf16's largest finite value, so that a value beyond it (and an infinity, which then travels in the tail) does not become inf - inf.
+#include <type_traits>
+#include "avcap_internal.h"
+#include "linear.h"
+
+namespace avc { namespace lin {
+
+#if defined(AVC_LIN_F32)
+typedef float elem_t;
+#define AVC_LAUNCH launch_tile_f32
+#elif defined(AVC_LIN_F16)
+typedef _Float16 elem_t;
+#define AVC_LAUNCH launch_tile_f16
+#else
+typedef __bf16 elem_t;
+#define AVC_LAUNCH launch_tile_bf16
+#endif
+
+namespace {
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr bool IS_F32 = std::is_same<elem_t, float>::value;
+constexpr bool IS_F16 = std::is_same<elem_t, _Float16>::value;
+constexpr int NP = IS_F32 ? 3 : 1;                 // 16-bit planes per operand in LDS
+constexpr int BK = IS_F32 ? 32 : 64;               // k step
+typedef typename Vec8<elem_t>::type elem8;
+typedef typename std::conditional<IS_F16, f16x8, bf16x8>::type half8;        // what the matrix instruction takes
+
+__device__ __forceinline__ f32x4 mfma(half8 a, half8 b, f32x4 c)
+{
+    if constexpr (IS_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// ---- LDS layout of one operand's BR x BK tile (16-bit elements, pieces of 16 bytes) ---------------------------------------------------------------------------
+// k contiguous: row r holds its BK values in BK / 8 pieces; rows contiguous: row k holds the BR values of one k in BR / 8 pieces.  The pieces of a row are permuted by an XOR
+// with a function of the row so that the lanes of a fragment read fall on different banks; the permutation is applied to the global address, because a direct load writes
+// LDS in lane order.
+template <int BR, bool KC> struct Tile {
+    static constexpr int ROW_BYTES = KC ? BK * 2 : BR * 2;
+    static constexpr int PIECES = ROW_BYTES / 16;                       // per row
+    static constexpr int ROWS = KC ? BR : BK;
+    static constexpr int BYTES = ROWS * ROW_BYTES;
+    __device__ static __forceinline__ int swizzle(int row)
+    {
+        if constexpr (KC) return BK == 64 ? (row >> 1) & 7 : (row >> 2) & 3;
+        else return (((row & 3) | (((row >> 3) & 1) << 2)) << 1) & (PIECES - 1);
+    }
+    // byte of piece p of row `row`
+    __device__ static __forceinline__ int at(int row, int p) { return row * ROW_BYTES + ((p ^ swizzle(row)) << 4); }
+
+    // fragment t of the wave whose rows start at r0: the lane's 8 values of k step ks
+    __device__ static __forceinline__ half8 fragment(const char *base, int r0, int t, int ks, int lane)
+    {
+        const int l16 = lane & 15, q = lane >> 4;
+        if constexpr (KC) {
+            const int row = r0 + 16 * t + l16;
+            return *reinterpret_cast<const half8 *>(base + at(row, ks * 4 + q));
+        } else {
+            // ds_read_b64_tr_b16: within 16 lanes, lane 4 a + c supplies the address of 4 adjacent values of k row a, and lane i receives the 4 k values of column i
+            const int a = l16 >> 2, c = l16 & 3;
+            const int col = r0 + 16 * t + 4 * c;
+            s16x4 v[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int k = ks * 32 + 8 * q + 4 * h + a;
+                const char *p = base + at(k, col >> 3) + ((col & 4) << 1);
+                v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p);
+            }
+            s16x8 w = {v[0][0], v[0][1], v[0][2], v[0][3], v[1][0], v[1][1], v[1][2], v[1][3]};
+            return __builtin_bit_cast(half8, w);
+        }
+    }
+};
+
+// ---- global -> LDS ------------------------------------------------------------------------------------------------------------------------------------------
+// (a) direct: 16-byte pieces straight into LDS.  The host has checked that every piece lies wholly inside or outside of the operand and is 16-byte aligned; pieces outside get an
+//     offset past the buffer's end, for which the hardware writes zeros.
+constexpr unsigned OUTSIDE = 0x80000000u;
+
+template <int BR, bool KC, int NW> struct Direct {
+    typedef Tile<BR, KC> L;
+    static constexpr int N = L::BYTES / 1024 / NW;                      // loads per wave
+    static constexpr int RPL = 1024 / L::ROW_BYTES;                     // rows per load
+    static_assert(N >= 1 && L::BYTES % (1024 * NW) == 0 && RPL >= 1, "tile does not divide into the waves' loads");
+    unsigned voff[N];
+    const char *base;
+    int64_t step_bytes, ld_bytes, left;                                 // bytes from `base` to the operand's end
+    __device__ __forceinline__ void init(const Operand &o, int64_t row0, int64_t rows, int64_t k0, int64_t K, int wave, int lane)
+    {
+        ld_bytes = o.ld * 2;
+        const int64_t first = KC ? row0 * o.ld + k0 : k0 * o.ld + row0, last = KC ? (rows - 1) * o.ld + K : (K - 1) * o.ld + rows;
+        base = (const char *)o.p + first * 2;
+        left = (last - first) * 2;
+        step_bytes = KC ? BK * 2 : BK * ld_bytes;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int r = (i * NW + wave) * RPL + lane / L::PIECES, p = (lane % L::PIECES) ^ L::swizzle(r);
+            voff[i] = (unsigned)(r * ld_bytes + p * 16);
+            if (KC ? row0 + r >= rows : row0 + p * 8 >= rows) voff[i] = OUTSIDE;
+        }
+    }
+    // the pieces of the step that starts at the current base, `kleft` values of k from it on
+    __device__ __forceinline__ void issue(char *lds, int64_t kleft, int wave, int lane)
+    {
+        __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)min(left, (int64_t)0x7fffffff), 0x00020000);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            unsigned v = voff[i];
+            if (kleft < BK) {
+                const int r = (i * NW + wave) * RPL + lane / L::PIECES, p = (lane % L::PIECES) ^ L::swizzle(r);
+                if (KC ? p * 8 >= kleft : r >= kleft) v = OUTSIDE;
+            }
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void *)(lds + (i * NW + wave) * 1024), 16, (int)v, 0, 0, 0);
+        }
+        base += step_bytes;
+        left -= step_bytes;
+    }
+};
+
+// (b) through registers: any alignment, any row length; float32 is split into its three planes on the way into LDS.
+__device__ __forceinline__ void split3(const f32x8 &x, bf16x8 out[3])
+{
+    constexpr float TOP = 3.3895313892515355e38f;                       // bf16's largest finite value
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const __bf16 h = (__bf16)__builtin_amdgcn_fmed3f(x[j], -TOP, TOP);
+        const float r = x[j] - (float)h;
+        const __bf16 m = (__bf16)__builtin_amdgcn_fmed3f(r, -TOP, TOP);
+        out[0][j] = h;
+        out[1][j] = m;
+        out[2][j] = (__bf16)(r - (float)m);
+    }
+}
+
+template <int BR, bool KC, int NT> struct Staged {
+    typedef Tile<BR, KC> L;
+    static constexpr int N = (L::BYTES / 16 + NT - 1) / NT;             // pieces of 8 values per thread
+    static constexpr bool FULL = L::BYTES / 16 % NT == 0;
+    elem8 v[N];
+    const elem_t *base;                                                 // element (row0, k0)
+    int64_t ld, rows;                                                   // rows left from row0 on
+    __device__ __forceinline__ void init(const Operand &o, int64_t row0, int64_t nrows, int64_t k0)
+    {
+        ld = o.ld;
+        rows = nrows - row0;
+        base = (const elem_t *)o.p + (KC ? row0 * ld + k0 : k0 * ld + row0);
+    }
+    __device__ __forceinline__ void load(int64_t kleft, int tid)
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int id = i * NT + tid, r = id / L::PIECES, p = id % L::PIECES;
+            const int64_t inner = (KC ? kleft : rows) - p * 8;          // values left along the contiguous axis
+            const bool row_in = (KC ? r < rows : r < kleft) && (FULL || id < L::BYTES / 16);
+            const elem_t *src = base + (int64_t)r * ld + p * 8;
+            elem8 x = {};
+            if (row_in && inner >= 8) __builtin_memcpy(&x, src, sizeof x);
+            else if (row_in && inner > 0) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (j < inner) x[j] = src[j];
+            }
+            v[i] = x;
+        }
+        base += KC ? (int64_t)BK : BK * ld;
+    }
+    __device__ __forceinline__ void store(char *lds, int tid) const
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int id = i * NT + tid, r = id / L::PIECES, p = id % L::PIECES;
+            if (!FULL && id >= L::BYTES / 16) continue;
+            char *dst = lds + L::at(r, p);
+            if constexpr (IS_F32) {
+                bf16x8 s[3];
+                split3(v[i], s);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) *reinterpret_cast<bf16x8 *>(dst + k * L::BYTES) = s[k];
+            } else {
+                *reinterpret_cast<elem8 *>(dst) = v[i];
+            }
+        }
+    }
+};
+
+// ---- the tile's products ------------------------------------------------------------------------------------------------------------------------------------
+template <int FM, int FN, typename LP, typename LQ>
+__device__ __forceinline__ void compute(const char *P, const char *Q, int pr0, int qr0, int lane, f32x4 (&acc)[FM][FN])
+{
+#pragma unroll
+    for (int ks = 0; ks < BK / 32; ++ks) {
+#pragma unroll
+        for (int a = 0; a < NP; ++a) {                                  // plane of Q: h with h m l, m with h m, l with h
+            half8 q[FN];
+#pragma unroll
+            for (int t = 0; t < FN; ++t) q[t] = LQ::fragment(Q + a * LQ::BYTES, qr0, t, ks, lane);
+#pragma unroll
+            for (int b = 0; b < NP - a; ++b)
+#pragma unroll
+                for (int i = 0; i < FM; ++i) {
+                    const half8 p = LP::fragment(P + b * LP::BYTES, pr0, i, ks, lane);
+#pragma unroll
+                    for (int t = 0; t < FN; ++t) acc[i][t] = mfma(q[t], p, acc[i][t]);
+                }
+        }
+    }
+}
+
+template <int VEC> __device__ __forceinline__ void store_run(elem_t *dst, const float *v, int64_t left, bool vec)
+{
+    if (vec && left >= VEC) {
+        typedef elem_t ev __attribute__((ext_vector_type(VEC)));
+        ev o;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) o[j] = (elem_t)v[j];
+        *reinterpret_cast<ev *>(dst) = o;
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            if (j < left) dst[j] = (elem_t)v[j];
+    }
+}
+
+template <int BM, int BN, int WM, int WN, bool PKC, bool QKC, bool DMA>
+__global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const TileArgs a)
+{
+    constexpr int NW = WM * WN, NT = NW * 64, FM = BM / WM / 16, FN = BN / WN / 16;
+    typedef Tile<BM, PKC> LP;
+    typedef Tile<BN, QKC> LQ;
+    constexpr int STAGE = NP * (LP::BYTES + LQ::BYTES);
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+    // Workgroups go to the 8 XCDs in turn; give every XCD a contiguous run of tiles, walked in bands of 8 tile rows, so that its L2 sees the same rows and columns again.
+    unsigned id = blockIdx.x;
+    {
+        const unsigned total = gridDim.x, per = total >> 3, rem = total & 7, x = id & 7;
+        id = x * per + min(x, rem) + (id >> 3);
+    }
+    const unsigned tiles = (unsigned)a.tiles_m * (unsigned)a.tiles_n, split = id / tiles, t = id % tiles;
+    const unsigned band = t / (8u * (unsigned)a.tiles_n), in_band = t % (8u * (unsigned)a.tiles_n), band_rows = min(8u, (unsigned)a.tiles_m - band * 8u);
+    const int64_t m0 = (int64_t)(band * 8u + in_band % band_rows) * BM, n0 = (int64_t)(in_band / band_rows) * BN;
+    const int64_t k0 = (int64_t)split * a.kper, kend = min(a.K, k0 + a.kper);
+    const int steps = (int)((kend - k0 + BK - 1) / BK);
+    const int pr0 = (wave / WN) * (BM / WM), qr0 = (wave % WN) * (BN / WN);
+
+    f32x4 acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    if constexpr (DMA) {
+        Direct<BM, PKC, NW> dp;
+        Direct<BN, QKC, NW> dq;
+        dp.init(a.P, m0, a.M, k0, a.K, wave, lane);
+        dq.init(a.Q, n0, a.N, k0, a.K, wave, lane);
+        if (steps > 0) {
+            dp.issue(smem, kend - k0, wave, lane);
+            dq.issue(smem + LP::BYTES, kend - k0, wave, lane);
+        }
+        for (int s = 0; s < steps; ++s) {
+            // this wave's pieces of step s are in LDS and its reads of step s - 1 are done; the barrier publishes the ones and frees the other buffer
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            char *cur = smem + (s & 1) * STAGE, *nxt = smem + ((s + 1) & 1) * STAGE;
+            if (s + 1 < steps) {
+                const int64_t kleft = kend - k0 - (int64_t)(s + 1) * BK;
+                dp.issue(nxt, kleft, wave, lane);
+                dq.issue(nxt + LP::BYTES, kleft, wave, lane);
+            }
+            compute<FM, FN, LP, LQ>(cur, cur + LP::BYTES, pr0, qr0, lane, acc);
+        }
+    } else {
+        Staged<BM, PKC, NT> sp;
+        Staged<BN, QKC, NT> sq;
+        sp.init(a.P, m0, a.M, k0);
+        sq.init(a.Q, n0, a.N, k0);
+        if (steps > 0) {
+            sp.load(kend - k0, tid);
+            sq.load(kend - k0, tid);
+        }
+        for (int s = 0; s < steps; ++s) {
+            char *cur = smem + (s & 1) * STAGE;
+            sp.store(cur, tid);
+            sq.store(cur + NP * LP::BYTES, tid);
+            __syncthreads();
+            if (s + 1 < steps) {
+                const int64_t kleft = kend - k0 - (int64_t)(s + 1) * BK;
+                sp.load(kleft, tid);
+                sq.load(kleft, tid);
+            }
+            compute<FM, FN, LP, LQ>(cur, cur + NP * LP::BYTES, pr0, qr0, lane, acc);
+        }
+    }
+
+    // ---- epilogue
+    const int64_t mw = m0 + pr0, nw = n0 + qr0;                         // the wave's corner
+    if (a.splits > 1) {
+        float *part = a.partial + (int64_t)split * a.M * a.N;
+        const bool vec = (a.N & 3) == 0;
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            const int64_t m = mw + 16 * i + (lane & 15);
+            if (m >= a.M) continue;
+#pragma unroll
+            for (int f = 0; f < FN; ++f) {
+                const int64_t n = nw + 16 * f + 4 * (lane >> 4);
+                float *dst = part + m * a.N + n;
+                if (vec && n + 4 <= a.N) *reinterpret_cast<f32x4 *>(dst) = acc[i][f];
+                else
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (n + j < a.N) dst[j] = acc[i][f][j];
+            }
+        }
+        return;
+    }
+    constexpr int VEC = 16 / sizeof(elem_t), WCOLS = BN / WN, PITCH = WCOLS * 4 + 16, LPR = WCOLS / VEC, RPI = 64 / LPR, ITER = 32 / RPI;
+    static_assert(NW * 32 * PITCH <= 2 * STAGE, "the epilogue's rows do not fit LDS");
+    typedef elem_t run_t __attribute__((ext_vector_type(VEC)));
+    const Epilogue &e = a.ep;
+    const bool vec_out = (a.ldo % VEC) == 0 && ((uintptr_t)a.out & 15) == 0, vec_z = (e.ldz % VEC) == 0 && ((uintptr_t)e.z & 15) == 0,
+               vec_res = (e.ldr % VEC) == 0 && ((uintptr_t)e.res & 15) == 0;
+    const int col = lane % LPR * VEC;
+    const int64_t n = nw + col, left = a.N - n;
+    float bias[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) bias[j] = e.bias && j < left ? (float)((const elem_t *)e.bias)[n + j] : 0.f;
+    __syncthreads();                                                    // the last step's reads of LDS are over
+    char *own = smem + wave * 32 * PITCH;
+#pragma unroll 1
+    for (int h = 0; h < FM / 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+            if (i / 2 == h) {
+#pragma unroll
+                for (int f = 0; f < FN; ++f) *reinterpret_cast<f32x4 *>(own + (16 * (i & 1) + (lane & 15)) * PITCH + (16 * f + 4 * (lane >> 4)) * 4) = acc[i][f];
+            }
+        __builtin_amdgcn_wave_barrier();
+        run_t res[ITER];
+#pragma unroll
+        for (int it = 0; it < ITER; ++it) {
+            const int64_t m = mw + 32 * h + it * RPI + lane / LPR;
+            res[it] = run_t(0);
+            if (e.res && m < a.M && left > 0) {
+                const elem_t *r = (const elem_t *)e.res + m * e.ldr + n;
+                if (vec_res && left >= VEC) res[it] = *reinterpret_cast<const run_t *>(r);
+                else
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j)
+                        if (j < left) res[it][j] = r[j];
+            }
+        }
+#pragma unroll
+        for (int it = 0; it < ITER; ++it) {
+            const int row = it * RPI + lane / LPR;
+            const int64_t m = mw + 32 * h + row;
+            float v[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; j += 4) {
+                const f32x4 x = *reinterpret_cast<const f32x4 *>(own + row * PITCH + (col + j) * 4);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[j + k] = x[k] + bias[j + k];
+            }
+            if (m >= a.M || left <= 0) continue;
+            if (e.z) store_run<VEC>((elem_t *)e.z + m * e.ldz + n, v, left, vec_z);
+            act_run<VEC>(v, e.act, e.slope);
+            if (e.res)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[j] += (float)res[it][j];
+            store_run<VEC>((elem_t *)a.out + m * a.ldo + n, v, left, vec_out);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+template <int BM, int BN, int WM, int WN, bool PKC, bool QKC, bool DMA> int launch_one(const TileArgs &a, hipStream_t s)
+{
+    constexpr int LDS = 2 * NP * (Tile<BM, PKC>::BYTES + Tile<BN, QKC>::BYTES);
+    static_assert(LDS <= 160 * 1024, "tile does not fit LDS");
+    auto k = tile_kernel<BM, BN, WM, WN, PKC, QKC, DMA>;
+    if (LDS > 64 * 1024) AVC_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+    hipLaunchKernelGGL(k, dim3((unsigned)((int64_t)a.tiles_m * a.tiles_n * a.splits)), dim3(WM * WN * 64), LDS, s, a);
+    AVC_HIP(hipGetLastError());
+    return AVC_OK;
+}
+
+template <int BM, int BN, int WM, int WN, bool DMA> int launch_layout(const TileArgs &a, hipStream_t s)
+{
+    if (a.P.kc) return a.Q.kc ? launch_one<BM, BN, WM, WN, true, true, DMA>(a, s) : launch_one<BM, BN, WM, WN, true, false, DMA>(a, s);
+    return a.Q.kc ? launch_one<BM, BN, WM, WN, false, true, DMA>(a, s) : launch_one<BM, BN, WM, WN, false, false, DMA>(a, s);
+}
+
+template <bool DMA> int launch_shape(const TileArgs &a, int tile, hipStream_t s)
+{
+    if (tile == TILE_BIG) {
+        if constexpr (IS_F32) return launch_layout<256, 128, 4, 2, DMA>(a, s);
+        else return launch_layout<256, 256, 2, 4, DMA>(a, s);
+    }
+    if (tile == TILE_MID) return launch_layout<128, 128, 2, 2, DMA>(a, s);
+    return launch_layout<64, 64, 2, 2, DMA>(a, s);
+}
+
+// the direct loads' conditions: whole 16-byte pieces, aligned, and a tile's offsets within 31 bits
+bool direct_ok(const Operand &o, int64_t rows, int64_t K)
+{
+    const int64_t inner = o.kc ? K : rows;
+    return ((uintptr_t)o.p & 15) == 0 && o.ld % 8 == 0 && inner % 8 == 0 && o.ld < (int64_t)1 << 21;
+}
+
+}  // namespace
+
+int AVC_LAUNCH(const TileArgs &a, int tile, hipStream_t s)
+{
+    if constexpr (!IS_F32)
+        if (direct_ok(a.P, a.M, a.K) && direct_ok(a.Q, a.N, a.K)) return launch_shape<true>(a, tile, s);
+    return launch_shape<false>(a, tile, s);
+}
+
+}}  // namespace avc::lin

@@ -1,0 +1,218 @@
+"""The layers an MLP is made of as differentiable calls on the HIP library: the dense layer with bias, activation and residual in its epilogue, and the layer norm.
+
+    y = linear(x, weight, bias, act='relu', residual=r)        y = act(x W^T + b) + r
+    y = layer_norm(x, weight, bias)                            y = (x - mean) / sqrt(var + eps) * g + b over the last axis
+
+`linear` is what one step of the reference's `MLP.forward` does (network/mlp.py:56-72: a Conv1d(k=1) and its activation), for any widths; network/mlp.py calls it.  Tensors are
+float32, bfloat16 or float16, all of one call alike, on the HIP device; there is no CPU path.  Both run on the current stream of the tensors' device, whichever device is current,
+take their workspace from torch's allocator (so a captured graph keeps its own) and have a backward pass of the same kernels (csrc/linear.hip, linear_tile.hip, layer_norm.hip).
+No gradient of a gradient.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _lib
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}                 # avc_dtype
+ACTS = {None: 0, 'relu': 1, 'leaky_relu': 2, 'soft_plus': 3, 'sigmoid': 4, 'tanh': 5, 'gelu': 6, 'silu': 7}   # avc_act
+
+
+def _check(who, first, **others):
+    if not isinstance(first, torch.Tensor):
+        raise TypeError(f'{who}: x: expected a torch.Tensor, got {type(first).__name__}')
+    if not first.is_cuda:
+        raise RuntimeError(f'{who} runs on the HIP device only; there is no CPU path (x lives on {first.device})')
+    if first.dtype not in DTYPES:
+        raise TypeError(f'{who}: float32, bfloat16 or float16, got {first.dtype}')
+    for name, t in others.items():
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f'{who}: {name}: expected a torch.Tensor, got {type(t).__name__}')
+        if t.dtype != first.dtype:
+            raise TypeError(f'{who}: {name} is {t.dtype}, x is {first.dtype}')
+        if t.device != first.device:
+            raise RuntimeError(f'{who}: {name} lives on {t.device}, x on {first.device}')
+
+
+def _rows(t):
+    """`t` (rows, columns) with adjacent columns, copied if they are not; rows may lie any distance apart."""
+    if t.stride(1) == 1 or t.shape[1] == 1:
+        return t if t.stride(0) >= 0 else t.contiguous()
+    return t.contiguous()
+
+
+def _row_stride(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _matrix(x):
+    """`x` (rows, columns) and its strides, one of which is 1: rows of adjacent values, or channel-first (a transposed view).  Copied otherwise."""
+    m, k = x.shape
+    if k == 1 or x.stride(1) == 1:
+        return x, _row_stride(x), 1
+    if x.stride(0) == 1 and m > 1:
+        return x, 1, x.stride(1)
+    x = x.contiguous()
+    return x, k, 1
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _space(nbytes, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _linear_forward(x, w, bias, res, act, slope, want_z):
+    m, k = x.shape
+    n = w.shape[0]
+    L, dev, dt = _lib.lib(), x.device, DTYPES[x.dtype]
+    x, xr, xc = _matrix(x)
+    w = _rows(w)
+    y = torch.empty((m, n), dtype=x.dtype, device=dev)
+    z = torch.empty_like(y) if want_z else None
+    nbytes = C.c_int64()
+    _lib.check(L.avc_linear_workspace(m, n, k, dt, xr, xc, C.byref(nbytes)))
+    ws = _space(nbytes.value, dev)
+    _lib.check(L.avc_linear(_lib.ctx(dev), x.data_ptr(), xr, xc, w.data_ptr(), _row_stride(w), _ptr(bias), _ptr(res), 0 if res is None else _row_stride(res), act, slope, m, n, k, dt,
+                            y.data_ptr(), n, _ptr(z), n, _ptr(ws), nbytes.value, _lib.stream_ptr(dev)))
+    return y, z
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, res, act, slope):
+        # relu and leaky_relu leave the sign of z in y: z is kept only where y does not have it
+        from_y = act in (1, 2) and res is None
+        y, z = _linear_forward(x, w, bias, res, act, slope, want_z=act != 0 and not from_y)
+        ctx.save_for_backward(x, w, y if from_y else z)
+        ctx.act, ctx.slope = act, slope
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, w, saved = ctx.saved_tensors
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        (m, k), n = x.shape, w.shape[0]
+        dev, dt = dy.device, DTYPES[dy.dtype]
+        dx = dw = db = None
+        if need_x or need_w or need_b:
+            L = _lib.lib()
+            g = _rows(dy)
+            x, xr, xc = _matrix(x)
+            w = _rows(w)
+            if need_x:
+                dx = torch.empty((m, k), dtype=dy.dtype, device=dev)
+            if need_w:
+                dw = torch.empty((n, k), dtype=dy.dtype, device=dev)
+            if need_b:
+                db = torch.empty((n,), dtype=dy.dtype, device=dev)
+            nbytes = C.c_int64()
+            _lib.check(L.avc_linear_backward_workspace(m, n, k, dt, C.byref(nbytes)))
+            ws = _space(nbytes.value, dev)
+            _lib.check(L.avc_linear_backward(_lib.ctx(dev), g.data_ptr(), _row_stride(g), x.data_ptr(), xr, xc, w.data_ptr(), _row_stride(w), _ptr(saved), n, ctx.act, ctx.slope, m, n, k, dt,
+                                             _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes.value, _lib.stream_ptr(dev)))
+        return dx, dw, db, dy if need_r else None, None, None
+
+
+def linear(x, weight, bias=None, act=None, slope=0.02, residual=None):
+    """act(x W^T + b) + residual in one pass.
+
+    x (..., K); weight (N, K), or (N, K, 1) as Conv1d(k=1) keeps it; bias (N); residual (..., N) -> (..., N).  act: None, 'relu', 'leaky_relu' (z > 0 ? z : slope z, slope >= 0),
+    'soft_plus' (torch's threshold of 20), 'sigmoid', 'tanh', 'gelu' (z Phi(z), not the tanh form), 'silu'.  x may be a transposed view (channel-first points) or any slice with one
+    unit stride; other layouts are copied.  Sums are float32 and each output is rounded once; float32 products keep 24 bits."""
+    if act not in ACTS:
+        raise ValueError(f'linear: unknown activation {act!r}, known are {[a for a in ACTS if a]}')
+    _check('linear', x, weight=weight, bias=bias, residual=residual)
+    if weight.dim() == 3 and weight.shape[2] == 1:
+        weight = weight[:, :, 0]
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f'linear: x {tuple(x.shape)} does not fit weight {tuple(weight.shape)}')
+    n, k = weight.shape
+    if n < 1 or k < 1:
+        raise ValueError(f'linear: a weight of shape {tuple(weight.shape)} has no values')
+    if bias is not None and tuple(bias.shape) != (n,):
+        raise ValueError(f'linear: bias {tuple(bias.shape)} for {n} outputs')
+    if residual is not None and residual.shape != x.shape[:-1] + (n,):
+        raise ValueError(f'linear: residual {tuple(residual.shape)}, the output is {tuple(x.shape[:-1]) + (n,)}')
+    slope = float(slope)
+    if act == 'leaky_relu' and not 0.0 <= slope < float('inf'):
+        raise ValueError(f'linear: leaky_relu takes a finite slope >= 0, got {slope}')
+    x2 = x if x.dim() == 2 else x.reshape(-1, k)
+    r2 = None if residual is None else _rows(residual if residual.dim() == 2 else residual.reshape(-1, n))
+    if bias is not None and n > 1 and bias.stride(0) != 1:
+        bias = bias.contiguous()
+    code = ACTS[act]
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or (residual is not None and residual.requires_grad)):
+        y = _Linear.apply(x2, weight, bias, r2, code, slope)
+    else:
+        y, _ = _linear_forward(x2, weight, bias, r2, code, slope, want_z=False)
+    return y if x.dim() == 2 else y.reshape(x.shape[:-1] + (n,))
+
+
+def _norm_forward(x, g, b, eps, want_stats):
+    m, c = x.shape
+    dev = x.device
+    x = _rows(x)
+    y = torch.empty((m, c), dtype=x.dtype, device=dev)
+    stats = torch.empty((2, m), dtype=torch.float32, device=dev) if want_stats else None
+    p = _ptr(stats)
+    _lib.check(_lib.lib().avc_layer_norm(_lib.ctx(dev), x.data_ptr(), _row_stride(x), _ptr(g), _ptr(b), eps, m, c, DTYPES[x.dtype], y.data_ptr(), c, p, p + 4 * m if p else p,
+                                         _lib.stream_ptr(dev)))
+    return y, stats
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, g, b, eps):
+        y, stats = _norm_forward(x, g, b, eps, want_stats=True)
+        ctx.save_for_backward(x, g, stats)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, g, stats = ctx.saved_tensors
+        need_x, need_g, need_b = ctx.needs_input_grad[:3]
+        m, c = x.shape
+        L, dev, dt = _lib.lib(), dy.device, DTYPES[dy.dtype]
+        x, dy = _rows(x), _rows(dy)
+        dx = torch.empty((m, c), dtype=dy.dtype, device=dev) if need_x else None
+        dg = torch.empty((c,), dtype=dy.dtype, device=dev) if need_g else None
+        db = torch.empty((c,), dtype=dy.dtype, device=dev) if need_b else None
+        nbytes = C.c_int64()
+        if need_g or need_b:
+            _lib.check(L.avc_layer_norm_backward_workspace(m, c, dt, C.byref(nbytes)))
+        ws = _space(nbytes.value, dev)
+        p = stats.data_ptr()
+        _lib.check(L.avc_layer_norm_backward(_lib.ctx(dev), dy.data_ptr(), _row_stride(dy), x.data_ptr(), _row_stride(x), _ptr(g), p, p + 4 * m, m, c, dt, _ptr(dx), c, _ptr(dg), _ptr(db),
+                                             _ptr(ws), nbytes.value, _lib.stream_ptr(dev)))
+        return dx, dg, db, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """The layer norm over the last axis: x (..., C), weight and bias (C) or None -> (..., C).  Mean and biased variance in float32, the variance from centred values."""
+    _check('layer_norm', x, weight=weight, bias=bias)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f'layer_norm: x {tuple(x.shape)} has no values along its last axis')
+    c = x.shape[-1]
+    for name, t in (('weight', weight), ('bias', bias)):
+        if t is not None and tuple(t.shape) != (c,):
+            raise ValueError(f'layer_norm: {name} {tuple(t.shape)} for rows of {c}')
+    eps = float(eps)
+    if not 0.0 <= eps < float('inf'):
+        raise ValueError(f'layer_norm: eps must be finite and >= 0, got {eps}')
+    x2 = x if x.dim() == 2 else x.reshape(-1, c)
+    weight, bias = (t if t is None or c == 1 or t.stride(0) == 1 else t.contiguous() for t in (weight, bias))
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+        y = _LayerNorm.apply(x2, weight, bias, eps)
+    else:
+        y, _ = _norm_forward(x2, weight, bias, eps, want_stats=False)
+    return y if x.dim() == 2 else y.reshape(x.shape)

@@ -17,7 +17,7 @@
  *     bound feature maps, per-column tables and mesh scratch are shared by the calls made on it,
  *     so two queries of one context must not overlap on different streams (use one context per
  *     concurrent stream, or order the streams with events).
- *   - all arithmetic is float32 in / float32 out; indices are int32 (faces) / int64 (KNN).
+ *   - all arithmetic is float32 in / float32 out (but for the dense layer and the layer norm below, which take 16-bit types too); indices are int32 (faces) / int64 (KNN).
  */
 #ifndef AVCAP_H
 #define AVCAP_H
@@ -150,6 +150,40 @@ int avc_hgfilter_debug_tensor(avc_ctx *ctx, int launch, int which, float *out_nc
  * x_dev, y_dev (N, C, HW) contiguous float32 (y_dev may equal x_dev); gamma_dev, beta_dev (C) or NULL. */
 int avc_group_norm(avc_ctx *ctx, const float *x_dev, int N, int C, int64_t HW, int G, const float *gamma_dev,
                    const float *beta_dev, float eps, int relu, float *y_dev, avc_stream stream);
+
+/* ---- dense layer and layer norm, forward and backward ---------------------------------------------
+ * The layers an MLP is made of (network/mlp.py:5-72 MLP: Conv1d(k=1) + activation), for any widths, with their gradients.  Tensors are device pointers of ONE element type
+ * `dtype`; sums, statistics and activations are float32, every output is rounded once.  Strides count ELEMENTS.  These calls keep nothing in the context: calls on
+ * several streams may overlap, and a captured graph owns whatever workspace its caller passed.  They leave the calling thread's current device as it was.
+ * `workspace` (16-byte aligned device memory, at least the bytes the matching _workspace call reports; NULL when that is 0) is free again when the call's work is done. */
+enum avc_dtype { AVC_F32 = 0, AVC_BF16 = 1, AVC_F16 = 2 };
+enum avc_act { AVC_ACT_NONE = 0, AVC_ACT_RELU = 1, AVC_ACT_LEAKY_RELU = 2 /* z > 0 ? z : slope z */, AVC_ACT_SOFTPLUS = 3 /* log(1 + e^z), z itself beyond 20 */,
+               AVC_ACT_SIGMOID = 4, AVC_ACT_TANH = 5, AVC_ACT_GELU = 6 /* z Phi(z) */, AVC_ACT_SILU = 7 };
+
+/* z = x w^T + bias, y = act(z) + res.
+ *   x (M, K) at x[m * x_row + k * x_col], one of the two strides being 1 (x_col = 1: rows of points; x_row = 1: channel-first points as Conv1d has them)
+ *   w (N, K) rows of K adjacent values, ldw apart;  bias (N) or NULL;  res (M, N), ldr apart, or NULL
+ *   y (M, N), ldy apart;  z (M, N), ldz apart, or NULL: the value before the activation, which the backward pass reads.  y, z overlap no input (y may be res itself).
+ * M >= 0, N, K >= 1.  A NaN or infinity of x or w reaches exactly the outputs it has a part in. */
+int avc_linear_workspace(int64_t M, int64_t N, int64_t K, int dtype, int64_t x_row, int64_t x_col, int64_t *bytes);
+int avc_linear(avc_ctx *ctx, const void *x, int64_t x_row, int64_t x_col, const void *w, int64_t ldw, const void *bias, const void *res, int64_t ldr, int act, float slope, int64_t M,
+               int64_t N, int64_t K, int dtype, void *y, int64_t ldy, void *z, int64_t ldz, void *workspace, int64_t workspace_bytes, avc_stream stream);
+
+/* dz = dy act'(z);  dx = dz w (M, K), dw = dz^T x (N, K), db = column sums of dz (N), each contiguous, any of them NULL.  (The gradient of res is dy.)
+ *   dy (M, N), lddy apart;  saved (M, N), ld_saved apart: z of the forward call; for AVC_ACT_RELU and AVC_ACT_LEAKY_RELU (slope >= 0) y of a call without res serves as well;
+ *   NULL for AVC_ACT_NONE.  x, w as in the forward call (x may be NULL without dw, w without dx).  dz is rounded to `dtype` once, as the operand of the two products. */
+int avc_linear_backward_workspace(int64_t M, int64_t N, int64_t K, int dtype, int64_t *bytes);
+int avc_linear_backward(avc_ctx *ctx, const void *dy, int64_t lddy, const void *x, int64_t x_row, int64_t x_col, const void *w, int64_t ldw, const void *saved, int64_t ld_saved, int act,
+                        float slope, int64_t M, int64_t N, int64_t K, int dtype, void *dx, void *dw, void *db, void *workspace, int64_t workspace_bytes, avc_stream stream);
+
+/* y = (x - mean) / sqrt(var + eps) * gamma + beta per row of C values (biased variance);  x, y (M, C) rows ldx / ldy apart (y may be x), gamma, beta (C) or NULL;
+ * mean, rstd (M) float32, both or neither: the statistics, which the backward pass reads.  M >= 0, C >= 1, eps >= 0. */
+int avc_layer_norm(avc_ctx *ctx, const void *x, int64_t ldx, const void *gamma, const void *beta, float eps, int64_t M, int64_t C, int dtype, void *y, int64_t ldy, float *mean, float *rstd,
+                   avc_stream stream);
+/* dx (M, C), lddx apart, dgamma (C), dbeta (C), any of them NULL; the workspace is needed for dgamma / dbeta only. */
+int avc_layer_norm_backward_workspace(int64_t M, int64_t C, int dtype, int64_t *bytes);
+int avc_layer_norm_backward(avc_ctx *ctx, const void *dy, int64_t lddy, const void *x, int64_t ldx, const void *gamma, const float *mean, const float *rstd, int64_t M, int64_t C, int dtype,
+                            void *dx, int64_t lddx, void *dgamma, void *dbeta, void *workspace, int64_t workspace_bytes, avc_stream stream);
 
 /* ---- queries -------------------------------------------------------------------------------
  * OccupancyNet.query (network/arch_avatar.py:356-381) = WarpingField.query (:113-140) +
