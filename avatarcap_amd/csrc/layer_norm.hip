@@ -18,30 +18,32 @@ namespace {
 
 template <typename T> struct Width { static constexpr int V = 16 / sizeof(T); };
 
-// V values of a row from column c on, zeros past the end.  Any alignment.
-template <typename T> __device__ __forceinline__ void load_run(const T *row, int64_t c, int64_t C, float *out)
+// A lane's run of V adjacent columns.  The run that the row ends in, and those past the end, are moved back to end with the row, so that every lane loads whole runs of any
+// alignment without a branch (a branch around a load makes each load wait for the one before); `first` is where the lane's own columns begin in it, V if it has none.  C >= V.
+template <int V> struct Run {
+    int64_t at;
+    int first;
+    __device__ __forceinline__ Run(int64_t col, int64_t C) : at(min(col, C - V)), first((int)min(col - min(col, C - V), (int64_t)V)) {}
+};
+
+template <int V, typename T> __device__ __forceinline__ void load_run(const T *row, int64_t at, float *out)
 {
-    constexpr int V = Width<T>::V;
     T v[V];
-    if (c + V <= C) __builtin_memcpy(v, row + c, sizeof v);
-    else
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = c + j < C ? row[c + j] : (T)0.f;
+    __builtin_memcpy(v, row + at, sizeof v);
 #pragma unroll
     for (int j = 0; j < V; ++j) out[j] = (float)v[j];
 }
 
-template <typename T> __device__ __forceinline__ void store_run(T *row, int64_t c, int64_t C, const float *in)
+template <int V, typename T> __device__ __forceinline__ void store_run(T *row, const Run<V> &run, const float *in)
 {
-    constexpr int V = Width<T>::V;
     T v[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = (T)in[j];
-    if (c + V <= C) __builtin_memcpy(row + c, v, sizeof v);
+    if (run.first == 0) __builtin_memcpy(row + run.at, v, sizeof v);
     else
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (c + j < C) row[c + j] = v[j];
+        for (int j = 1; j < V; ++j)
+            if (j >= run.first) row[run.at + j] = v[j];
 }
 
 // sum over the tpr threads of a row; TPR = 0: a runtime power of two up to the wave
@@ -62,47 +64,67 @@ template <int TPR> __device__ __forceinline__ float row_sum(float v, int tpr, fl
     }
 }
 
-template <typename T, int TPR, int NCH>
+// R rows at a time per set of lanes, so that a lane has several loads in flight
+template <typename T, int V, int TPR, int NCH, int R>
 __global__ __launch_bounds__(TPR ? TPR : 256) void norm_kernel(const T *__restrict__ x, int64_t ldx, const T *__restrict__ g, const T *__restrict__ b, float eps, int64_t M, int64_t C, int tpr_log,
                                                               T *y, int64_t ldy, float *mean_out, float *rstd_out)
 {
-    constexpr int V = Width<T>::V;
     __shared__ float red[16];
     const int tpr = TPR ? TPR : 1 << tpr_log, lane = threadIdx.x & (tpr - 1), rows = TPR ? 1 : 256 >> tpr_log, sub = TPR ? 0 : threadIdx.x >> tpr_log;
-    for (int64_t m0 = (int64_t)blockIdx.x * rows; m0 < M; m0 += (int64_t)gridDim.x * rows) {
-        const int64_t m = m0 + sub;
-        const bool in = m < M;                                               // TPR = 0 only: the other lanes of the wave still need the shuffles
-        const T *row = x + (in ? m : 0) * ldx;
-        float v[NCH][V], s = 0.f;
+    const float inv = 1.f / (float)C;
+    for (int64_t m0 = (int64_t)blockIdx.x * rows * R; m0 < M; m0 += (int64_t)gridDim.x * rows * R) {
+        float v[R][NCH][V], mean[R], rstd[R];
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            load_run(row, ((int64_t)c * tpr + lane) * V, C, v[c]);
+        for (int r = 0; r < R; ++r) {                                    // rows past the end repeat the last one: the other lanes of the wave still need the shuffles
+            const T *row = x + min(m0 + r * rows + sub, M - 1) * ldx;
 #pragma unroll
-            for (int j = 0; j < V; ++j) s += v[c][j];
+            for (int c = 0; c < NCH; ++c) load_run<V>(row, Run<V>(((int64_t)c * tpr + lane) * V, C).at, v[r][c]);
         }
-        const float inv = 1.f / (float)C, mean = row_sum<TPR>(s, tpr, red) * inv;
-        s = 0.f;
 #pragma unroll
-        for (int c = 0; c < NCH; ++c)
+        for (int r = 0; r < R; ++r) {
+            float s = 0.f;
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                v[c][j] -= mean;
-                if (((int64_t)c * tpr + lane) * V + j < C) s += v[c][j] * v[c][j];
+            for (int c = 0; c < NCH; ++c) {
+                const int first = Run<V>(((int64_t)c * tpr + lane) * V, C).first;
+#pragma unroll
+                for (int j = 0; j < V; ++j) s += j >= first ? v[r][c][j] : 0.f;
             }
-        const float rstd = 1.f / sqrtf(row_sum<TPR>(s, tpr, red) * inv + eps);
-        if (!in) continue;
+            mean[r] = row_sum<TPR>(s, tpr, red) * inv;
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float s = 0.f;
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                const int first = Run<V>(((int64_t)c * tpr + lane) * V, C).first;
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    v[r][c][j] -= mean[r];
+                    s += j >= first ? v[r][c][j] * v[r][c][j] : 0.f;
+                }
+            }
+            rstd[r] = 1.f / sqrtf(row_sum<TPR>(s, tpr, red) * inv + eps);
+        }
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
-            const int64_t col = ((int64_t)c * tpr + lane) * V;
-            if (col >= C) continue;
+            const Run<V> run(((int64_t)c * tpr + lane) * V, C);
             float gg[V], bb[V];
-            if (g) load_run(g, col, C, gg);
-            if (b) load_run(b, col, C, bb);
+            if (g) load_run<V>(g, run.at, gg);
+            if (b) load_run<V>(b, run.at, bb);
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[c][j] = v[c][j] * rstd * (g ? gg[j] : 1.f) + (b ? bb[j] : 0.f);
-            store_run(y + m * ldy, col, C, v[c]);
+            for (int r = 0; r < R; ++r) {
+                const int64_t m = m0 + r * rows + sub;
+                if (m >= M) continue;
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[r][c][j] = v[r][c][j] * rstd[r] * (g ? gg[j] : 1.f) + (b ? bb[j] : 0.f);
+                store_run<V>(y + m * ldy, run, v[r][c]);
+            }
         }
-        if (mean_out && lane == 0) { mean_out[m] = mean; rstd_out[m] = rstd; }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int64_t m = m0 + r * rows + sub;
+            if (mean_out && lane == 0 && m < M) { mean_out[m] = mean[r]; rstd_out[m] = rstd[r]; }
+        }
     }
 }
 
@@ -117,46 +139,46 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(const T *__restrict__ x
         const T *row = x + m * ldx;
         float v[V], s = 0.f;
         for (int64_t c = (int64_t)threadIdx.x * V; c < C; c += 1024 * V) {
-            load_run(row, c, C, v);
+            const Run<V> run(c, C);
+            load_run<V>(row, run.at, v);
 #pragma unroll
-            for (int j = 0; j < V; ++j) s += v[j];
+            for (int j = 0; j < V; ++j) s += j >= run.first ? v[j] : 0.f;
         }
         const float mean = row_sum<1024>(s, 1024, red) / (float)C;
         s = 0.f;
         for (int64_t c = (int64_t)threadIdx.x * V; c < C; c += 1024 * V) {
-            load_run(row, c, C, v);
+            const Run<V> run(c, C);
+            load_run<V>(row, run.at, v);
 #pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (c + j < C) s += (v[j] - mean) * (v[j] - mean);
+            for (int j = 0; j < V; ++j) s += j >= run.first ? (v[j] - mean) * (v[j] - mean) : 0.f;
         }
         const float rstd = 1.f / sqrtf(row_sum<1024>(s, 1024, red) / (float)C + eps);
         for (int64_t c = (int64_t)threadIdx.x * V; c < C; c += 1024 * V) {
             float gg[V], bb[V];
-            load_run(row, c, C, v);
-            if (g) load_run(g, c, C, gg);
-            if (b) load_run(b, c, C, bb);
+            const Run<V> run(c, C);
+            load_run<V>(row, run.at, v);
+            if (g) load_run<V>(g, run.at, gg);
+            if (b) load_run<V>(b, run.at, bb);
 #pragma unroll
             for (int j = 0; j < V; ++j) v[j] = (v[j] - mean) * rstd * (g ? gg[j] : 1.f) + (b ? bb[j] : 0.f);
-            store_run(y + m * ldy, c, C, v);
+            store_run<V>(y + m * ldy, run, v);
         }
         if (mean_out && threadIdx.x == 0) { mean_out[m] = mean; rstd_out[m] = rstd; }
     }
 }
 
-template <typename T, int TPR, int NCH>
+template <typename T, int V, int TPR, int NCH>
 __global__ __launch_bounds__(TPR ? TPR : 256) void norm_backward_kernel(const T *__restrict__ dy, int64_t lddy, const T *__restrict__ x, int64_t ldx, const T *__restrict__ g,
                                                                        const float *__restrict__ mean_in, const float *__restrict__ rstd_in, int64_t M, int64_t C, int tpr_log, T *dx, int64_t lddx,
                                                                        float *part)
 {
-    constexpr int V = Width<T>::V, E = NCH * V;
     __shared__ float red[TPR ? 16 : 256 * (V + 1)];
     const int tpr = TPR ? TPR : 1 << tpr_log, lane = threadIdx.x & (tpr - 1), rows = TPR ? 1 : 256 >> tpr_log, sub = TPR ? 0 : threadIdx.x >> tpr_log;
     const float inv = 1.f / (float)C;
     float gg[NCH][V], dg[NCH][V], db[NCH][V];
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-        const int64_t col = ((int64_t)c * tpr + lane) * V;
-        if (g) load_run(g, col, C, gg[c]);
+        if (g) load_run<V>(g, Run<V>(((int64_t)c * tpr + lane) * V, C).at, gg[c]);
 #pragma unroll
         for (int j = 0; j < V; ++j) { dg[c][j] = db[c][j] = 0.f; if (!g) gg[c][j] = 1.f; }
     }
@@ -166,41 +188,41 @@ __global__ __launch_bounds__(TPR ? TPR : 256) void norm_backward_kernel(const T 
         float xv[NCH][V], t[NCH][V];
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
-            const int64_t col = ((int64_t)c * tpr + lane) * V;
-            load_run(x + m * ldx, col, C, xv[c]);
-            load_run(dy + m * lddy, col, C, t[c]);
+            const int64_t at = Run<V>(((int64_t)c * tpr + lane) * V, C).at;
+            load_run<V>(x + m * ldx, at, xv[c]);
+            load_run<V>(dy + m * lddy, at, t[c]);
         }
         const float mean = mean_in[m], rstd = rstd_in[m];
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-        for (int c = 0; c < NCH; ++c)
+        for (int c = 0; c < NCH; ++c) {
+            const int first = Run<V>(((int64_t)c * tpr + lane) * V, C).first;
 #pragma unroll
-            for (int j = 0; j < V; ++j) {                                // past the row's end dy is zero, and with it every sum
+            for (int j = 0; j < V; ++j) {
                 const float xh = (xv[c][j] - mean) * rstd;
                 if (in) { dg[c][j] += t[c][j] * xh; db[c][j] += t[c][j]; }
                 t[c][j] *= gg[c][j];
                 xv[c][j] = xh;
-                s1 += t[c][j];
-                s2 += t[c][j] * xh;
+                s1 += j >= first ? t[c][j] : 0.f;
+                s2 += j >= first ? t[c][j] * xh : 0.f;
             }
+        }
         if (!dx) continue;
         s1 = row_sum<TPR>(s1, tpr, red) * inv;
         s2 = row_sum<TPR>(s2, tpr, red) * inv;
         if (!in) continue;
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
-            const int64_t col = ((int64_t)c * tpr + lane) * V;
-            if (col >= C) continue;
 #pragma unroll
             for (int j = 0; j < V; ++j) t[c][j] = rstd * (t[c][j] - s1 - xv[c][j] * s2);
-            store_run(dx + m * lddx, col, C, t[c]);
+            store_run<V>(dx + m * lddx, Run<V>(((int64_t)c * tpr + lane) * V, C), t[c]);
         }
     }
     if (!part) return;
     float *out = part + (int64_t)blockIdx.x * 2 * C;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-        const int64_t col = ((int64_t)c * tpr + lane) * V;
+        const Run<V> run(((int64_t)c * tpr + lane) * V, C);
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
             float(&v)[V] = which ? db[c] : dg[c];
@@ -217,7 +239,7 @@ __global__ __launch_bounds__(TPR ? TPR : 256) void norm_backward_kernel(const T 
             if (sub == 0)
 #pragma unroll
                 for (int j = 0; j < V; ++j)
-                    if (col + j < C) out[which * C + col + j] = v[j];
+                    if (j >= run.first) out[which * C + run.at + j] = v[j];
         }
     }
 }
@@ -232,25 +254,27 @@ __global__ __launch_bounds__(1024) void norm_backward_long_kernel(const T *__res
         const float mean = mean_in[m], rstd = rstd_in[m];
         float xv[V], t[V], gg[V], s1 = 0.f, s2 = 0.f;
         for (int64_t c = (int64_t)threadIdx.x * V; c < C; c += 1024 * V) {
-            load_run(x + m * ldx, c, C, xv);
-            load_run(dy + m * lddy, c, C, t);
-            if (g) load_run(g, c, C, gg);
+            const Run<V> run(c, C);
+            load_run<V>(x + m * ldx, run.at, xv);
+            load_run<V>(dy + m * lddy, run.at, t);
+            if (g) load_run<V>(g, run.at, gg);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const float u = t[j] * (g ? gg[j] : 1.f);
-                s1 += u;
-                s2 += u * ((xv[j] - mean) * rstd);
+                s1 += j >= run.first ? u : 0.f;
+                s2 += j >= run.first ? u * ((xv[j] - mean) * rstd) : 0.f;
             }
         }
         s1 = row_sum<1024>(s1, 1024, red) / (float)C;
         s2 = row_sum<1024>(s2, 1024, red) / (float)C;
         for (int64_t c = (int64_t)threadIdx.x * V; c < C; c += 1024 * V) {
-            load_run(x + m * ldx, c, C, xv);
-            load_run(dy + m * lddy, c, C, t);
-            if (g) load_run(g, c, C, gg);
+            const Run<V> run(c, C);
+            load_run<V>(x + m * ldx, run.at, xv);
+            load_run<V>(dy + m * lddy, run.at, t);
+            if (g) load_run<V>(g, run.at, gg);
 #pragma unroll
             for (int j = 0; j < V; ++j) t[j] = rstd * (t[j] * (g ? gg[j] : 1.f) - s1 - (xv[j] - mean) * rstd * s2);
-            store_run(dx + m * lddx, c, C, t);
+            store_run<V>(dx + m * lddx, run, t);
         }
     }
 }
@@ -263,10 +287,11 @@ __global__ __launch_bounds__(256) void norm_columns_kernel(const T *__restrict__
     constexpr int V = Width<T>::V;
     const int64_t col = ((int64_t)blockIdx.y * 256 + threadIdx.x) * V, m1 = min(M, ((int64_t)blockIdx.x + 1) * rows_per);
     if (col >= C) return;
+    const Run<V> run(col, C);
     float dg[V] = {}, db[V] = {}, xv[V], t[V];
     for (int64_t m = (int64_t)blockIdx.x * rows_per; m < m1; ++m) {
-        load_run(x + m * ldx, col, C, xv);
-        load_run(dy + m * lddy, col, C, t);
+        load_run<V>(x + m * ldx, run.at, xv);
+        load_run<V>(dy + m * lddy, run.at, t);
         const float mean = mean_in[m], rstd = rstd_in[m];
 #pragma unroll
         for (int j = 0; j < V; ++j) { dg[j] += t[j] * ((xv[j] - mean) * rstd); db[j] += t[j]; }
@@ -274,26 +299,27 @@ __global__ __launch_bounds__(256) void norm_columns_kernel(const T *__restrict__
     float *out = part + (int64_t)blockIdx.x * 2 * C;
 #pragma unroll
     for (int j = 0; j < V; ++j)
-        if (col + j < C) { out[col + j] = dg[j]; out[C + col + j] = db[j]; }
+        if (j >= run.first) { out[run.at + j] = dg[j]; out[C + run.at + j] = db[j]; }
 }
 
 constexpr int64_t MAX_GRID = 1 << 20;                                   // the kernels walk rows beyond it
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// How a row of C values is spread: the smallest set of threads whose registers (two chunks each) hold it.
-struct Spread { int tpr, nch, tpr_log; };                                // tpr = 0: too long
+// How a row of C values is spread: the smallest set of threads whose registers (up to four chunks each) hold it.
+struct Spread { int tpr, nch, tpr_log; bool narrow; };                   // tpr = 0: too long; narrow: rows shorter than a run, one value per lane
 Spread spread_of(int64_t C, int dtype)
 {
     const int V = dtype == AVC_F32 ? 4 : 8;
     const int64_t runs = cdiv(C, V);
+    if (C < V) return Spread{8, 1, 3, true};
     if (runs <= 128) {
         int lg = 3;
         while (lg < 6 && (1 << lg) < runs) ++lg;
-        return Spread{1 << lg, runs > 64 ? 2 : 1, lg};
+        return Spread{1 << lg, runs > 64 ? 2 : 1, lg, false};
     }
-    if (runs <= 512) return Spread{256, runs > 256 ? 2 : 1, 8};
-    if (runs <= 2048) return Spread{1024, runs > 1024 ? 2 : 1, 10};
-    return Spread{0, 0, 0};
+    if (runs <= 1024) return Spread{256, runs > 512 ? 4 : runs > 256 ? 2 : 1, 8, false};
+    if (runs <= 2048) return Spread{1024, 2, 10, false};
+    return Spread{0, 0, 0, false};
 }
 
 // workgroups of the backward pass (strips of the column sums)
@@ -308,19 +334,20 @@ int64_t backward_blocks(int64_t M, int64_t C, int dtype)
 template <typename T> int norm_forward(const void *x, int64_t ldx, const void *g, const void *b, float eps, int64_t M, int64_t C, int dtype, void *y, int64_t ldy, float *mean, float *rstd,
                                        hipStream_t s)
 {
+    constexpr int W = Width<T>::V;
     const Spread sp = spread_of(C, dtype);
-#define AVC_NORM(TPR, NCH, GRID, BLOCK)                                                                                                                          \
-    hipLaunchKernelGGL((norm_kernel<T, TPR, NCH>), dim3((unsigned)std::min<int64_t>(GRID, MAX_GRID)), dim3(BLOCK), 0, s, (const T *)x, ldx, (const T *)g, (const T *)b, eps, M, C, sp.tpr_log, (T *)y, ldy, mean, rstd)
-    if (sp.tpr == 0)
+#define AVC_NORM(V, TPR, NCH, R, BLOCK)                                                                                                                             \
+    hipLaunchKernelGGL((norm_kernel<T, V, TPR, NCH, R>), dim3((unsigned)std::min<int64_t>(cdiv(M, (R) * (TPR ? 1 : 256 / sp.tpr)), MAX_GRID)), dim3(BLOCK), 0, s, (const T *)x, ldx,                \
+                       (const T *)g, (const T *)b, eps, M, C, sp.tpr_log, (T *)y, ldy, mean, rstd)
+    if (sp.narrow) AVC_NORM(1, 0, 1, 1, 256);
+    else if (sp.tpr == 0)
         hipLaunchKernelGGL(norm_long_kernel<T>, dim3((unsigned)std::min<int64_t>(M, MAX_GRID)), dim3(1024), 0, s, (const T *)x, ldx, (const T *)g, (const T *)b, eps, M, C, (T *)y, ldy, mean, rstd);
     else if (sp.tpr <= 64) {
-        const int64_t grid = cdiv(M, 256 / sp.tpr);
-        if (sp.nch == 1) AVC_NORM(0, 1, grid, 256); else AVC_NORM(0, 2, grid, 256);
+        if (M < 8192) { if (sp.nch == 1) AVC_NORM(W, 0, 1, 1, 256); else AVC_NORM(W, 0, 2, 1, 256); }
+        else { if (sp.nch == 1) AVC_NORM(W, 0, 1, 4, 256); else AVC_NORM(W, 0, 2, 2, 256); }
     } else if (sp.tpr == 256) {
-        if (sp.nch == 1) AVC_NORM(256, 1, M, 256); else AVC_NORM(256, 2, M, 256);
-    } else {
-        if (sp.nch == 1) AVC_NORM(1024, 1, M, 1024); else AVC_NORM(1024, 2, M, 1024);
-    }
+        if (sp.nch == 1) AVC_NORM(W, 256, 1, 1, 256); else if (sp.nch == 2) AVC_NORM(W, 256, 2, 1, 256); else AVC_NORM(W, 256, 4, 1, 256);
+    } else AVC_NORM(W, 1024, 2, 1, 1024);
 #undef AVC_NORM
     AVC_HIP(hipGetLastError());
     return AVC_OK;
@@ -332,21 +359,21 @@ template <typename T> int norm_backward(const void *dy, int64_t lddy, const void
     const Spread sp = spread_of(C, dtype);
     const int64_t blocks = backward_blocks(M, C, dtype);
     float *p = dg || db ? part : nullptr;
-#define AVC_NORM(TPR, NCH, BLOCK)                                                                                                                                \
-    hipLaunchKernelGGL((norm_backward_kernel<T, TPR, NCH>), dim3((unsigned)blocks), dim3(BLOCK), 0, s, (const T *)dy, lddy, (const T *)x, ldx, (const T *)g, mean, rstd, M, C, sp.tpr_log,       \
+    constexpr int W = Width<T>::V;
+#define AVC_NORM(V, TPR, NCH, BLOCK)                                                                                                                                \
+    hipLaunchKernelGGL((norm_backward_kernel<T, V, TPR, NCH>), dim3((unsigned)blocks), dim3(BLOCK), 0, s, (const T *)dy, lddy, (const T *)x, ldx, (const T *)g, mean, rstd, M, C, sp.tpr_log,       \
                        (T *)dx, lddx, p)
-    if (sp.tpr == 0) {
+    if (sp.narrow) AVC_NORM(1, 0, 1, 256);
+    else if (sp.tpr == 0) {
         if (dx && M) hipLaunchKernelGGL(norm_backward_long_kernel<T>, dim3((unsigned)std::min<int64_t>(M, MAX_GRID)), dim3(1024), 0, s, (const T *)dy, lddy, (const T *)x, ldx, (const T *)g, mean, rstd, M, C, (T *)dx, lddx);
         if (p)
             hipLaunchKernelGGL(norm_columns_kernel<T>, dim3((unsigned)blocks, (unsigned)cdiv(C, 256 * Width<T>::V)), dim3(256), 0, s, (const T *)dy, lddy, (const T *)x, ldx, mean, rstd, M, C,
                                cdiv(M, blocks), p);
     } else if (sp.tpr <= 64) {
-        if (sp.nch == 1) AVC_NORM(0, 1, 256); else AVC_NORM(0, 2, 256);
+        if (sp.nch == 1) AVC_NORM(W, 0, 1, 256); else AVC_NORM(W, 0, 2, 256);
     } else if (sp.tpr == 256) {
-        if (sp.nch == 1) AVC_NORM(256, 1, 256); else AVC_NORM(256, 2, 256);
-    } else {
-        if (sp.nch == 1) AVC_NORM(1024, 1, 1024); else AVC_NORM(1024, 2, 1024);
-    }
+        if (sp.nch == 1) AVC_NORM(W, 256, 1, 256); else if (sp.nch == 2) AVC_NORM(W, 256, 2, 256); else AVC_NORM(W, 256, 4, 256);
+    } else AVC_NORM(W, 1024, 2, 1024);
 #undef AVC_NORM
     AVC_HIP(hipGetLastError());
     if (p) return launch_colsum2(p, (int)blocks, C, dtype, dg, db, s);

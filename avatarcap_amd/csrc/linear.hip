@@ -39,13 +39,21 @@ template <typename T> struct FewArgs { const T *S; int64_t lds; const T *F; int6
 
 template <typename T> struct Chunk { static constexpr int LANE = 32 / sizeof(T), K = 4 * LANE; typedef T vec __attribute__((ext_vector_type(LANE))); vec v; };
 
-template <typename T> __device__ __forceinline__ Chunk<T> load_chunk(const T *row, int64_t k, int64_t K)
+template <typename T> __device__ __forceinline__ Chunk<T> load_chunk(const T *row, int64_t k)
 {
     Chunk<T> c;
-    if (k + Chunk<T>::LANE <= K) __builtin_memcpy(&c.v, row + k, sizeof c.v);
-    else
+    __builtin_memcpy(&c.v, row + k, sizeof c.v);
+    return c;
+}
+// the chunk that K ends in: values past the end are zero
+template <typename T> __device__ __forceinline__ Chunk<T> load_tail(const T *row, int64_t k, int64_t K)
+{
+    Chunk<T> c;
 #pragma unroll
-        for (int j = 0; j < Chunk<T>::LANE; ++j) c.v[j] = k + j < K ? row[k + j] : (T)0.f;
+    for (int j = 0; j < Chunk<T>::LANE; ++j) c.v[j] = row[min(k + j, K - 1)];
+#pragma unroll
+    for (int j = 0; j < Chunk<T>::LANE; ++j)
+        if (k + j >= K) c.v[j] = (T)0.f;
     return c;
 }
 
@@ -83,21 +91,26 @@ template <typename T, int FB> __global__ __launch_bounds__(1024) void few_kernel
 #pragma unroll
     for (int b = 0; b < FB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
     constexpr int CK = Chunk<T>::K, U = 4;
-    const int64_t stride = (int64_t)a.kw * CK;
+    const int64_t stride = (int64_t)a.kw * CK, qk = q * Chunk<T>::LANE;
     int64_t k = (int64_t)kslot * CK;
     for (; k + (U - 1) * stride + CK <= a.K; k += U * stride) {
         Chunk<T> s[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) s[u] = load_chunk(srow, k + u * stride + q * Chunk<T>::LANE, a.K);
+        for (int u = 0; u < U; ++u) s[u] = load_chunk(srow, k + u * stride + qk);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int b = 0; b < FB; ++b) acc[b] = chunk_mfma(s[u], load_chunk(frow[b], k + u * stride + q * Chunk<T>::LANE, a.K), acc[b]);
+            for (int b = 0; b < FB; ++b) acc[b] = chunk_mfma(s[u], load_chunk(frow[b], k + u * stride + qk), acc[b]);
     }
-    for (; k < a.K; k += stride) {
-        const Chunk<T> s = load_chunk(srow, k + q * Chunk<T>::LANE, a.K);
+    for (; k + CK <= a.K; k += stride) {
+        const Chunk<T> s = load_chunk(srow, k + qk);
 #pragma unroll
-        for (int b = 0; b < FB; ++b) acc[b] = chunk_mfma(s, load_chunk(frow[b], k + q * Chunk<T>::LANE, a.K), acc[b]);
+        for (int b = 0; b < FB; ++b) acc[b] = chunk_mfma(s, load_chunk(frow[b], k + qk), acc[b]);
+    }
+    if (k < a.K) {
+        const Chunk<T> s = load_tail(srow, k + qk, a.K);
+#pragma unroll
+        for (int b = 0; b < FB; ++b) acc[b] = chunk_mfma(s, load_tail(frow[b], k + qk, a.K), acc[b]);
     }
     if (a.kw > 1) {
 #pragma unroll
@@ -130,7 +143,11 @@ template <typename T, int NB> __global__ __launch_bounds__(256) void narrow_kern
     __shared__ float part[3][64][V * NB + 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t m = ((int64_t)blockIdx.x * 64 + lane) * V;
-    const bool full = m + V <= M;
+    int64_t at[V];                                                      // M < V: one by one
+#pragma unroll
+    for (int j = 0; j < V; ++j) at[j] = min(m + j, M - 1);
+    const bool full = M % V == 0;                                       // uniform
+    const int64_t mc = min(m, M - V);
     float acc[NB][V] = {};
     for (int64_t kb = 0; kb < K; kb += KT) {
         const int kt = (int)min((int64_t)KT, K - kb);
@@ -140,19 +157,24 @@ template <typename T, int NB> __global__ __launch_bounds__(256) void narrow_kern
             wk[k][n] = n < N && k < kt ? (float)w[n * ldw + kb + k] : 0.f;
         }
         __syncthreads();
-        if (m < M) {
+        if (full) {
 #pragma unroll 8
             for (int k = wave; k < kt; k += 4) {
-                const T *src = x + (kb + k) * ldx + m;
                 T v[V];
-                if (full) __builtin_memcpy(v, src, sizeof v);
-                else
-#pragma unroll
-                    for (int j = 0; j < V; ++j) v[j] = m + j < M ? src[j] : (T)0.f;
+                __builtin_memcpy(v, x + (kb + k) * ldx + mc, sizeof v);
 #pragma unroll
                 for (int n = 0; n < NB; ++n)
 #pragma unroll
                     for (int j = 0; j < V; ++j) acc[n][j] = fmaf((float)v[j], wk[k][n], acc[n][j]);
+            }
+        } else {
+#pragma unroll 4
+            for (int k = wave; k < kt; k += 4) {
+                const T *src = x + (kb + k) * ldx;
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) acc[n][j] = fmaf((float)src[at[j]], wk[k][n], acc[n][j]);
             }
         }
     }
@@ -220,19 +242,24 @@ template <typename T, int V> __global__ __launch_bounds__(256) void dact_kernel(
 
 }  // namespace
 
-// out(n) = sum over the strips of part[strip][n]: 32 columns and 8 runs of strips per workgroup, the runs' sums added in order.  Columns past N1 belong to the second output.
-template <typename T> __global__ __launch_bounds__(256) void colsum_kernel(const float *__restrict__ part, int strips, int64_t N, int64_t N1, T *out, T *out2)
+// out(n) = sum over the strips of part[strip][n]: 32 columns and 32 runs of strips per workgroup, the runs' sums added in order.  Columns past N1 belong to the second output.
+// A few hundred strips of a few hundred columns are too few bytes to matter; what counts is the chain of dependent loads, so 1024 threads share it (8 runs took 38 - 74 us for
+// 1024 - 2048 strips).
+template <typename T> __global__ __launch_bounds__(1024) void colsum_kernel(const float *__restrict__ part, int strips, int64_t N, int64_t N1, T *out, T *out2)
 {
-    __shared__ float red[8][33];
+    __shared__ float red[32][33];
     const int lx = threadIdx.x & 31, ly = threadIdx.x >> 5;
     const int64_t n = (int64_t)blockIdx.x * 32 + lx;
     float s = 0.f;
-    if (n < N)
-        for (int i = ly; i < strips; i += 8) s += part[(int64_t)i * N + n];
+    if (n < N) {
+#pragma unroll 8
+        for (int i = ly; i < strips; i += 32) s += part[(int64_t)i * N + n];
+    }
     red[ly][lx] = s;
     __syncthreads();
     if (ly || n >= N) return;
-    for (int y = 1; y < 8; ++y) s += red[y][lx];
+#pragma unroll
+    for (int y = 1; y < 32; ++y) s += red[y][lx];
     if (n < N1) { if (out) out[n] = (T)s; }
     else if (out2) out2[n - N1] = (T)s;
 }
@@ -240,9 +267,9 @@ template <typename T> __global__ __launch_bounds__(256) void colsum_kernel(const
 static int launch_columns(const float *part, int strips, int64_t N, int64_t N1, int dtype, void *out, void *out2, hipStream_t s)
 {
     const dim3 grid((unsigned)((N + 31) / 32));
-    if (dtype == AVC_F32) hipLaunchKernelGGL(colsum_kernel<float>, grid, dim3(256), 0, s, part, strips, N, N1, (float *)out, (float *)out2);
-    else if (dtype == AVC_BF16) hipLaunchKernelGGL(colsum_kernel<__bf16>, grid, dim3(256), 0, s, part, strips, N, N1, (__bf16 *)out, (__bf16 *)out2);
-    else hipLaunchKernelGGL(colsum_kernel<_Float16>, grid, dim3(256), 0, s, part, strips, N, N1, (_Float16 *)out, (_Float16 *)out2);
+    if (dtype == AVC_F32) hipLaunchKernelGGL(colsum_kernel<float>, grid, dim3(1024), 0, s, part, strips, N, N1, (float *)out, (float *)out2);
+    else if (dtype == AVC_BF16) hipLaunchKernelGGL(colsum_kernel<__bf16>, grid, dim3(1024), 0, s, part, strips, N, N1, (__bf16 *)out, (__bf16 *)out2);
+    else hipLaunchKernelGGL(colsum_kernel<_Float16>, grid, dim3(1024), 0, s, part, strips, N, N1, (_Float16 *)out, (_Float16 *)out2);
     AVC_HIP(hipGetLastError());
     return AVC_OK;
 }

@@ -161,22 +161,32 @@ template <int BR, bool KC, int NT> struct Staged {
         rows = nrows - row0;
         base = (const elem_t *)o.p + (KC ? row0 * ld + k0 : k0 * ld + row0);
     }
+    // No branch depends on a lane: a branch around a load would make every load wait for the one before it.  Rows past the end repeat the last one (their outputs are not
+    // stored); a step that ends inside a piece takes its values one by one, from clamped indices, and zeroes those past the end.
     __device__ __forceinline__ void load(int64_t kleft, int tid)
     {
+        const bool whole = KC ? kleft >= BK : (kleft >= BK && rows >= BR);
+        if (whole) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int id = i * NT + tid, r = id / L::PIECES, p = id % L::PIECES;
-            const int64_t inner = (KC ? kleft : rows) - p * 8;          // values left along the contiguous axis
-            const bool row_in = (KC ? r < rows : r < kleft) && (FULL || id < L::BYTES / 16);
-            const elem_t *src = base + (int64_t)r * ld + p * 8;
-            elem8 x = {};
-            if (row_in && inner >= 8) __builtin_memcpy(&x, src, sizeof x);
-            else if (row_in && inner > 0) {
+            for (int i = 0; i < N; ++i) {
+                const int id = i * NT + tid, r = id / L::PIECES, p = id % L::PIECES;
+                const int64_t row = KC ? min((int64_t)r, rows - 1) : (FULL ? r : min(r, BK - 1));
+                __builtin_memcpy(&v[i], base + row * ld + p * 8, sizeof v[i]);
+            }
+        } else {
+            const int64_t inner = KC ? kleft : rows, outer = KC ? rows : kleft;       // both >= 1
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int id = i * NT + tid, r = id / L::PIECES, p = id % L::PIECES;
+                const elem_t *src = base + min((int64_t)r, outer - 1) * ld;
+                elem8 x;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = src[min((int64_t)(p * 8 + j), inner - 1)];
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (j < inner) x[j] = src[j];
+                    if (p * 8 + j >= inner || r >= outer) x[j] = (elem_t)0.f;
+                v[i] = x;
             }
-            v[i] = x;
         }
         base += KC ? (int64_t)BK : BK * ld;
     }

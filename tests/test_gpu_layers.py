@@ -151,3 +151,62 @@ def test_large_tiles_and_splits(dtype):
     check_linear(40, 4096, 72, dtype, act='silu')                            # few tiles, a long sum: split
     check_linear(5000, 40, 24, dtype, act='leaky_relu')                      # the weight gradient splits over the rows
     check_linear(2050, 2050, 640, dtype, act='silu', grad=True)
+
+
+def check_norm(m, c, dtype, affine=True, eps=1e-5, scale=1.5, shift=0.25, pad=0, grad=True):
+    """Bounds: the row's sums are float32 over C values: mean to (C 2^-24) max|x| =: em, and with s = 1 / std, x^ = (x - mean) s to e = s em + 8 2^-24 (|x^| + 1) + (C + 8) 2^-24 |x^|
+    (the variance's own relative error, halved by the root, is below (C + 4) 2^-24 plus (em s)^2).  Gradients are sums of products of x^, dy and g over the row or the columns."""
+    gen = torch.Generator().manual_seed(m * 131 + c)
+    x = (torch.randn(m, c, generator=gen) * scale + shift).to(dtype)
+    g = (1 + 0.2 * torch.randn(c, generator=gen)).to(dtype) if affine else None
+    b = (0.1 * torch.randn(c, generator=gen)).to(dtype) if affine else None
+    dy = torch.randn(m, c, generator=gen).to(dtype)
+    buf = torch.full((m, c + pad), float('nan'), dtype=dtype, device='cuda')
+    buf[:, pad // 2:pad // 2 + c] = x.cuda()
+    xd, gd, bd = buf[:, pad // 2:pad // 2 + c].detach(), dev(g), dev(b)
+    if grad:
+        for t in (xd, gd, bd):
+            if t is not None:
+                t.requires_grad_()
+    X, DY, u = dbl(x), dbl(dy), unit(dtype)
+    G = torch.ones(c, dtype=torch.float64) if g is None else dbl(g)
+    B = torch.zeros(c, dtype=torch.float64) if b is None else dbl(b)
+    mean = X.mean(1, keepdim=True)
+    std = ((X - mean).pow(2).mean(1, keepdim=True) + eps).sqrt()
+    xh = (X - mean) / std
+    em = (c + 2) * E32 * X.abs().amax(1, keepdim=True)
+    e = em / std + (c + 16) * E32 * (xh.abs() + 1) + (em / std) ** 2 * xh.abs()
+    y = xh * G + B
+    tiny = torch.finfo(dtype).tiny
+    got = layer_norm(xd, gd, bd, eps=eps)
+    close(got, y, u * y.abs() + (1 + u) * (e * G.abs() + 4 * E32 * (xh * G).abs() + 2 * E32 * B.abs()) + tiny, 'y')
+    if not grad:
+        return
+    got.backward(dy.cuda())
+    t = DY * G
+    dx = (t - t.mean(1, keepdim=True) - xh * (t * xh).mean(1, keepdim=True)) / std
+    s1 = t.abs().mean(1, keepdim=True)
+    s2 = (t.abs() * (xh.abs() + e)).mean(1, keepdim=True)
+    err = ((c + 16) * E32 * (t.abs() + s1 + xh.abs() * s2) + e * s2 + xh.abs() * (t.abs() * e).mean(1, keepdim=True)) / std
+    rel = (c + 8) * E32 + (em / std) ** 2
+    close(xd.grad, dx, u * dx.abs() + (1 + u) * (err + rel * dx.abs()) + tiny, 'dx')
+    if affine:
+        dg, db = (DY * xh).sum(0), DY.sum(0)
+        close(gd.grad, dg, u * dg.abs() + (1 + u) * ((DY.abs() * e).sum(0) + (m + 4) * E32 * (DY * xh).abs().sum(0)) + tiny, 'dg')
+        close(bd.grad, db, u * db.abs() + (1 + u) * (m + 2) * E32 * DY.abs().sum(0) + tiny, 'db')
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('m,c', [(1, 1), (3, 2), (5, 3), (1, 7), (70, 8), (1, 9), (33, 31), (257, 64), (1, 256), (9000, 256), (9001, 70), (8193, 777), (66, 1023), (3, 1024), (40, 2049), (17, 4097),
+                                 (5, 8191), (3, 8193), (2, 16384), (3, 16385), (21, 20000)])
+def test_norm_sizes(m, c, dtype):
+    check_norm(m, c, dtype)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_norm_layouts_and_values(dtype):
+    check_norm(37, 100, dtype, affine=False)
+    check_norm(37, 101, dtype, pad=6)
+    check_norm(300, 16500, dtype, pad=3, grad=False)
+    check_norm(1200, 260, dtype, scale=0.01, shift=4.0 if dtype == torch.float32 else 0.02)
+    check_norm(7, 512, dtype, scale=100.0, shift=-50.0, eps=1.0)
