@@ -119,14 +119,16 @@ template <int BR, bool KC, int NW> struct Direct {
     __device__ __forceinline__ void issue(char *lds, int64_t kleft, int wave, int lane)
     {
         __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)min(left, (int64_t)0x7fffffff), 0x00020000);
+        if (kleft >= BK) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            unsigned v = voff[i];
-            if (kleft < BK) {
+            for (int i = 0; i < N; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void *)(lds + (i * NW + wave) * 1024), 16, (int)voff[i], 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
                 const int r = (i * NW + wave) * RPL + lane / L::PIECES, p = (lane % L::PIECES) ^ L::swizzle(r);
-                if (KC ? p * 8 >= kleft : r >= kleft) v = OUTSIDE;
+                const unsigned v = (KC ? p * 8 >= (int)kleft : r >= (int)kleft) ? OUTSIDE : voff[i];
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void *)(lds + (i * NW + wave) * 1024), 16, (int)v, 0, 0, 0);
             }
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void *)(lds + (i * NW + wave) * 1024), 16, (int)v, 0, 0, 0);
         }
         base += step_bytes;
         left -= step_bytes;
@@ -232,6 +234,29 @@ __device__ __forceinline__ void compute(const char *P, const char *Q, int pr0, i
     }
 }
 
+template <int F, typename L> __device__ __forceinline__ void read_fragments(half8 (&f)[F], const char *base, int r0, int ks, int lane)
+{
+#pragma unroll
+    for (int t = 0; t < F; ++t) f[t] = L::fragment(base, r0, t, ks, lane);
+}
+template <int FM, int FN> __device__ __forceinline__ void multiply(const half8 (&p)[FM], const half8 (&q)[FN], f32x4 (&acc)[FM][FN])
+{
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int t = 0; t < FN; ++t) acc[i][t] = mfma(q[t], p[i], acc[i][t]);
+}
+// deals READS LDS reads evenly among MFMAS matrix instructions of the surrounding block
+template <int READS, int MFMAS> __device__ __forceinline__ void interleave()
+{
+    constexpr int PER = MFMAS / READS > 0 ? MFMAS / READS : 1;
+#pragma unroll
+    for (int i = 0; i < READS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
+    }
+}
+
 template <int VEC> __device__ __forceinline__ void store_run(elem_t *dst, const float *v, int64_t left, bool vec)
 {
     if (vec && left >= VEC) {
@@ -247,13 +272,16 @@ template <int VEC> __device__ __forceinline__ void store_run(elem_t *dst, const 
     }
 }
 
+// Steps of LDS.  float32's middle tile keeps one (48 KB), so that three workgroups share a CU and fill each other's waits; everything else two.
+constexpr int stages(int BM) { return IS_F32 && BM == 128 ? 1 : 2; }
+
 template <int BM, int BN, int WM, int WN, bool PKC, bool QKC, bool DMA>
-__global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const TileArgs a)
+__global__ __launch_bounds__(WM * WN * 64, IS_F32 && BM == 128 ? 3 : 2) void tile_kernel(const TileArgs a)
 {
     constexpr int NW = WM * WN, NT = NW * 64, FM = BM / WM / 16, FN = BN / WN / 16;
     typedef Tile<BM, PKC> LP;
     typedef Tile<BN, QKC> LQ;
-    constexpr int STAGE = NP * (LP::BYTES + LQ::BYTES);
+    constexpr int STAGE = NP * (LP::BYTES + LQ::BYTES), STAGES = stages(BM);
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
@@ -281,22 +309,46 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const TileArgs a)
         Direct<BN, QKC, NW> dq;
         dp.init(a.P, m0, a.M, k0, a.K, wave, lane);
         dq.init(a.Q, n0, a.N, k0, a.K, wave, lane);
+        // Software pipeline: while the matrix instructions of one half of a step (32 k) run, the fragments of the next half are read from LDS, and the pieces of the step after
+        // next are on their way.  One barrier per step, between its halves: there every wave has read all of step s (so its buffer takes step s + 2) and every wave's pieces of
+        // step s + 1, asked for a whole step ago, have arrived.
+        static_assert(NP == 1 && BK == 64, "two halves of 32 k");
+        constexpr int READS = FM * (PKC ? 1 : 2) + FN * (QKC ? 1 : 2);
         if (steps > 0) {
             dp.issue(smem, kend - k0, wave, lane);
             dq.issue(smem + LP::BYTES, kend - k0, wave, lane);
-        }
-        for (int s = 0; s < steps; ++s) {
-            // this wave's pieces of step s are in LDS and its reads of step s - 1 are done; the barrier publishes the ones and frees the other buffer
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            char *cur = smem + (s & 1) * STAGE, *nxt = smem + ((s + 1) & 1) * STAGE;
-            if (s + 1 < steps) {
-                const int64_t kleft = kend - k0 - (int64_t)(s + 1) * BK;
-                dp.issue(nxt, kleft, wave, lane);
-                dq.issue(nxt + LP::BYTES, kleft, wave, lane);
+            if (steps > 1) {
+                dp.issue(smem + STAGE, kend - k0 - BK, wave, lane);
+                dq.issue(smem + STAGE + LP::BYTES, kend - k0 - BK, wave, lane);
             }
-            compute<FM, FN, LP, LQ>(cur, cur + LP::BYTES, pr0, qr0, lane, acc);
+            half8 p0[FM], q0[FN], p1[FM], q1[FN];
+            read_fragments<FN, LQ>(q0, smem + LP::BYTES, qr0, 0, lane);
+            read_fragments<FM, LP>(p0, smem, pr0, 0, lane);
+            for (int s = 0; s < steps; ++s) {
+                char *cur = smem + (s & 1) * STAGE, *nxt = smem + ((s + 1) & 1) * STAGE;
+                read_fragments<FN, LQ>(q1, cur + LP::BYTES, qr0, 1, lane);
+                read_fragments<FM, LP>(p1, cur, pr0, 1, lane);
+                multiply(p0, q0, acc);
+                interleave<READS, FM * FN>();
+                __builtin_amdgcn_sched_barrier(0);
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                if (s + 2 < steps) {
+                    const int64_t kleft = kend - k0 - (int64_t)(s + 2) * BK;
+                    dp.issue(cur, kleft, wave, lane);
+                    dq.issue(cur + LP::BYTES, kleft, wave, lane);
+                }
+                // (the last step reads what the other buffer holds and uses none of it)
+                read_fragments<FN, LQ>(q0, nxt + LP::BYTES, qr0, 0, lane);
+                read_fragments<FM, LP>(p0, nxt, pr0, 0, lane);
+                multiply(p1, q1, acc);
+                interleave<READS, FM * FN>();
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     } else {
         Staged<BM, PKC, NT> sp;
@@ -308,7 +360,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const TileArgs a)
             sq.load(kend - k0, tid);
         }
         for (int s = 0; s < steps; ++s) {
-            char *cur = smem + (s & 1) * STAGE;
+            char *cur = smem + (STAGES == 2 ? (s & 1) * STAGE : 0);
+            if (STAGES == 1 && s) __syncthreads();
             sp.store(cur, tid);
             sq.store(cur + NP * LP::BYTES, tid);
             __syncthreads();
@@ -344,7 +397,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const TileArgs a)
         return;
     }
     constexpr int VEC = 16 / sizeof(elem_t), WCOLS = BN / WN, PITCH = WCOLS * 4 + 16, LPR = WCOLS / VEC, RPI = 64 / LPR, ITER = 32 / RPI;
-    static_assert(NW * 32 * PITCH <= 2 * STAGE, "the epilogue's rows do not fit LDS");
+    static_assert(NW * 32 * PITCH <= STAGES * STAGE, "the epilogue's rows do not fit LDS");
     typedef elem_t run_t __attribute__((ext_vector_type(VEC)));
     const Epilogue &e = a.ep;
     const bool vec_out = (a.ldo % VEC) == 0 && ((uintptr_t)a.out & 15) == 0, vec_z = (e.ldz % VEC) == 0 && ((uintptr_t)e.z & 15) == 0,
@@ -404,7 +457,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const TileArgs a)
 
 template <int BM, int BN, int WM, int WN, bool PKC, bool QKC, bool DMA> int launch_one(const TileArgs &a, hipStream_t s)
 {
-    constexpr int LDS = 2 * NP * (Tile<BM, PKC>::BYTES + Tile<BN, QKC>::BYTES);
+    constexpr int LDS = stages(BM) * NP * (Tile<BM, PKC>::BYTES + Tile<BN, QKC>::BYTES);
     static_assert(LDS <= 160 * 1024, "tile does not fit LDS");
     auto k = tile_kernel<BM, BN, WM, WN, PKC, QKC, DMA>;
     if (LDS > 64 * 1024) AVC_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
