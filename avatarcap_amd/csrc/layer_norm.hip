@@ -170,7 +170,7 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(const T *__restrict__ x
 template <typename T, int V, int TPR, int NCH>
 __global__ __launch_bounds__(TPR ? TPR : 256) void norm_backward_kernel(const T *__restrict__ dy, int64_t lddy, const T *__restrict__ x, int64_t ldx, const T *__restrict__ g,
                                                                        const float *__restrict__ mean_in, const float *__restrict__ rstd_in, int64_t M, int64_t C, int tpr_log, T *dx, int64_t lddx,
-                                                                       float *part)
+                                                                       float *part, T *dg_out, T *db_out)
 {
     __shared__ float red[TPR ? 16 : 256 * (V + 1)];
     const int tpr = TPR ? TPR : 1 << tpr_log, lane = threadIdx.x & (tpr - 1), rows = TPR ? 1 : 256 >> tpr_log, sub = TPR ? 0 : threadIdx.x >> tpr_log;
@@ -239,7 +239,10 @@ __global__ __launch_bounds__(TPR ? TPR : 256) void norm_backward_kernel(const T 
             if (sub == 0)
 #pragma unroll
                 for (int j = 0; j < V; ++j)
-                    if (j >= run.first) out[which * C + run.at + j] = v[j];
+                    if (j >= run.first) {
+                        if (gridDim.x > 1) out[which * C + run.at + j] = v[j];
+                        else if (T *to = which ? db_out : dg_out) to[run.at + j] = (T)v[j];       // a single workgroup's sums are the gradients themselves
+                    }
         }
     }
 }
@@ -327,8 +330,9 @@ int64_t backward_blocks(int64_t M, int64_t C, int dtype)
 {
     const Spread s = spread_of(C, dtype);
     if (s.tpr == 0) return std::max<int64_t>(1, std::min<int64_t>(cdiv(M, 16), 64));
-    if (s.tpr <= 64) return std::max<int64_t>(1, std::min<int64_t>(cdiv(M, 256 / s.tpr), 1024));
-    return std::max<int64_t>(1, std::min<int64_t>(M, s.tpr == 256 ? 1024 : 512));
+    if (M <= 4 * std::max(1, 256 / s.tpr)) return 1;
+    if (s.tpr <= 64) return std::min<int64_t>(cdiv(M, 256 / s.tpr), 1024);
+    return std::min<int64_t>(M, s.tpr == 256 ? 1024 : 512);
 }
 
 template <typename T> int norm_forward(const void *x, int64_t ldx, const void *g, const void *b, float eps, int64_t M, int64_t C, int dtype, void *y, int64_t ldy, float *mean, float *rstd,
@@ -362,7 +366,7 @@ template <typename T> int norm_backward(const void *dy, int64_t lddy, const void
     constexpr int W = Width<T>::V;
 #define AVC_NORM(V, TPR, NCH, BLOCK)                                                                                                                                \
     hipLaunchKernelGGL((norm_backward_kernel<T, V, TPR, NCH>), dim3((unsigned)blocks), dim3(BLOCK), 0, s, (const T *)dy, lddy, (const T *)x, ldx, (const T *)g, mean, rstd, M, C, sp.tpr_log,       \
-                       (T *)dx, lddx, p)
+                       (T *)dx, lddx, p, (T *)dg, (T *)db)
     if (sp.narrow) AVC_NORM(1, 0, 1, 256);
     else if (sp.tpr == 0) {
         if (dx && M) hipLaunchKernelGGL(norm_backward_long_kernel<T>, dim3((unsigned)std::min<int64_t>(M, MAX_GRID)), dim3(1024), 0, s, (const T *)dy, lddy, (const T *)x, ldx, (const T *)g, mean, rstd, M, C, (T *)dx, lddx);
@@ -376,7 +380,7 @@ template <typename T> int norm_backward(const void *dy, int64_t lddy, const void
     } else AVC_NORM(W, 1024, 2, 1024);
 #undef AVC_NORM
     AVC_HIP(hipGetLastError());
-    if (p) return launch_colsum2(p, (int)blocks, C, dtype, dg, db, s);
+    if (p && (blocks > 1 || sp.tpr == 0)) return launch_colsum2(p, (int)blocks, C, dtype, dg, db, s);
     return AVC_OK;
 }
 

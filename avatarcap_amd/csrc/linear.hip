@@ -26,6 +26,7 @@ template <typename T> __global__ __launch_bounds__(256) void reduce_kernel(const
     const int64_t total = M * N;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         float v = 0.f;
+#pragma unroll 8
         for (int s = 0; s < splits; ++s) v += part[s * total + i];
         finish<T>(v, i / N, i % N, e, out, ldo);
     }
@@ -197,9 +198,9 @@ template <typename T, int NB> __global__ __launch_bounds__(256) void narrow_kern
 
 // ---- the activation's gradient dz = dy act'(z), and the column sums of dz in the same pass -------------------------------------------------------------------------
 // Lanes take V adjacent columns, `tx` lanes a row, 256 / tx rows at a time; every workgroup walks a strip of rows and leaves its column sums in part[strip][N] (float32, a
-// fixed order), which colsum_kernel adds.  dz is rounded to the element type: it is the operand of two matrix products in that type.
+// fixed order), which colsum_kernel adds (a single strip's sums are the bias gradient itself).  dz is rounded to the element type: it is the operand of two matrix products in that type.
 template <typename T, int V> __global__ __launch_bounds__(256) void dact_kernel(const T *__restrict__ dy, int64_t lddy, const T *__restrict__ z, int64_t ldz, int act, float slope, int64_t M, int64_t N,
-                                                                               int64_t rows_per, int tx, T *__restrict__ dz, float *__restrict__ part)
+                                                                               int64_t rows_per, int tx, T *__restrict__ dz, float *__restrict__ part, T *__restrict__ db)
 {
     typedef T vec __attribute__((ext_vector_type(V)));
     const int lx = threadIdx.x % tx, ly = threadIdx.x / tx, ty = 256 / tx;
@@ -227,7 +228,7 @@ template <typename T, int V> __global__ __launch_bounds__(256) void dact_kernel(
             for (int j = 0; j < V; ++j) sum[j] += v[j];
         }
     }
-    if (!part) return;
+    if (!part && !db) return;
     __shared__ float red[256][V + 1];
 #pragma unroll
     for (int j = 0; j < V; ++j) red[threadIdx.x][j] = sum[j];
@@ -237,7 +238,10 @@ template <typename T, int V> __global__ __launch_bounds__(256) void dact_kernel(
 #pragma unroll
         for (int j = 0; j < V; ++j) sum[j] += red[y * tx + lx][j];
 #pragma unroll
-    for (int j = 0; j < V; ++j) part[(int64_t)blockIdx.x * N + n + j] = sum[j];
+    for (int j = 0; j < V; ++j) {
+        if (db) db[n + j] = (T)sum[j];
+        else part[(int64_t)blockIdx.x * N + n + j] = sum[j];
+    }
 }
 
 }  // namespace
@@ -280,36 +284,61 @@ namespace {
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ---- which tile, how many splits: from the sizes alone, so that the workspace can be asked for in advance -----------------------------------------------------------
+// The time of a launch is estimated for every tile shape and a ladder of splits, and the least taken.  With W workgroups on the fullest CU, `occ` of them at a time, and S steps of
+// k each:   launch + max(ceil(W / occ) (S lone_step + lone), W (S step + rest)) + the splits' sums written, read and reduced.
+// `lone_*` is a workgroup's own latency, `step` / `rest` its share of a busy CU (matrix rate; writing the tile out).  Constants in us, fitted to 1020 timed launches of 17 shapes
+// (64 .. 262144 rows, 64 .. 4096 columns and k, all three products): the choice came out 2 % slower than the best of all tiles and splits in the mean, 38 % at worst (a 14 us call).
+struct TileCost { int occ; double lone_step, lone, step, rest; };
+constexpr TileCost COST_16[3] = {{1, 1.62, 7.0, 0.01, 11.1}, {2, 0.91, 1.9, 0.47, 3.3}, {5, 0.64, 0.0, 0.20, 1.0}};
+constexpr TileCost COST_F32[3] = {{1, 2.67, 5.4, 0.00, 12.0}, {3, 3.64, 1.7, 1.57, 4.3}, {3, 0.89, 1.7, 0.57, 1.0}};
+constexpr int SPLITS[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256};
+
 struct Plan { int tile, tiles_m, tiles_n, splits; int64_t kper; };
 
 Plan plan_tiles(int64_t M, int64_t N, int64_t K, int dtype)
 {
-    Plan p;
     const int bk = tile_bk(dtype);
-    auto count = [&](int t) { return cdiv(M, tile_bm(dtype, t)) * cdiv(N, tile_bn(dtype, t)); };
-    p.tile = M <= 64 || N <= 64 ? TILE_SMALL : (count(TILE_BIG) >= 192 && K >= 512 && N > 128 ? TILE_BIG : TILE_MID);
-    if (p.tile == TILE_MID && count(TILE_MID) * std::min<int64_t>(16, cdiv(K, 4 * bk)) < 128) p.tile = TILE_SMALL;
-    const int64_t tiles = count(p.tile);
-    p.tiles_m = (int)cdiv(M, tile_bm(dtype, p.tile));
-    p.tiles_n = (int)cdiv(N, tile_bn(dtype, p.tile));
-    int64_t splits = 1;
-    if (tiles < 256) splits = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512 / tiles, 256), K / (4 * bk)));
-    p.kper = cdiv(cdiv(K, splits), bk) * bk;
-    if (p.kper < bk) p.kper = bk;
-    p.splits = (int)std::max<int64_t>(1, cdiv(K, p.kper));
-    return p;
+    Plan best{};
+    double least = 0;
+    for (int tile = TILE_BIG; tile <= TILE_SMALL; ++tile) {
+        const int64_t tm = cdiv(M, tile_bm(dtype, tile)), tn = cdiv(N, tile_bn(dtype, tile));
+        const TileCost &c = (dtype == AVC_F32 ? COST_F32 : COST_16)[tile];
+        for (int want : SPLITS) {
+            if (want > 1 && (K < (int64_t)want * 2 * bk || (double)want * M * N > 1e8)) break;
+            const int64_t kper = std::max<int64_t>(bk, cdiv(cdiv(K, want), bk) * bk), splits = std::max<int64_t>(1, cdiv(K, kper)), W = cdiv(tm * tn * splits, 256);
+            const double S = (double)cdiv(std::min(kper, K), bk);
+            double us = std::max((double)cdiv(W, c.occ) * (S * c.lone_step + c.lone), (double)W * (S * c.step + c.rest));
+            if (splits > 1) us += 3 + 8e-6 / 5 * (double)splits * M * N;
+            if (!best.splits || us < least) {
+                least = us;
+                best = Plan{tile, (int)tm, (int)tn, (int)splits, kper};
+            }
+        }
+    }
+    return best;
 }
 size_t partial_bytes(const Plan &p, int64_t M, int64_t N) { return p.splits > 1 ? sizeof(float) * (size_t)p.splits * (size_t)M * (size_t)N : 0; }
 
-// strips of the activation-gradient pass: enough workgroups to fill the chip, at least 8 rows each
-int64_t strips_for(int64_t M, int64_t N) { return std::max<int64_t>(1, std::min<int64_t>(cdiv(M, 8), std::max<int64_t>(1, 2048 / cdiv(N, 1024)))); }
-
-inline size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 inline int esize(int dtype) { return dtype == AVC_F32 ? 4 : 2; }
 
+// lanes that share a row in the activation-gradient pass
+int lanes_for(int64_t N, int v)
+{
+    int tx = 1;
+    while (tx < 256 && (int64_t)tx * v < N) tx *= 2;
+    return tx;
+}
+// its strips of rows: eight rows per lane, and no more strips than fill the chip
+int64_t strips_for(int64_t M, int64_t N, int dtype)
+{
+    const int v = 16 / esize(dtype), tx = lanes_for(N, v);
+    return std::max<int64_t>(1, std::min<int64_t>(cdiv(M, 8 * (256 / tx)), std::max<int64_t>(1, 2048 / cdiv(N, (int64_t)tx * v))));
+}
+
+inline size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 template <typename T> int launch_reduce(const float *part, int splits, int64_t M, int64_t N, void *out, int64_t ldo, const Epilogue &e, hipStream_t s)
 {
-    const int64_t blocks = std::min<int64_t>(cdiv(M * N, 256), 4096);
+    const int64_t blocks = std::min<int64_t>(cdiv(M * N, 256), 8192);
     hipLaunchKernelGGL(reduce_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, part, splits, M, N, (T *)out, ldo, e);
     AVC_HIP(hipGetLastError());
     return AVC_OK;
@@ -365,17 +394,16 @@ Route route(int64_t M, int64_t N, bool x_kc)
     return ROUTE_TILE;
 }
 
-template <typename T> int launch_dact(const void *dy, int64_t lddy, const void *z, int64_t ldz, int act, float slope, int64_t M, int64_t N, void *dz, float *part, int64_t strips, hipStream_t s)
+template <typename T> int launch_dact(const void *dy, int64_t lddy, const void *z, int64_t ldz, int act, float slope, int64_t M, int64_t N, void *dz, float *part, void *db, int64_t strips, hipStream_t s)
 {
     constexpr int V = 16 / sizeof(T);
     const bool wide = N % V == 0 && lddy % V == 0 && ((uintptr_t)dy & 15) == 0 && (!z || (ldz % V == 0 && ((uintptr_t)z & 15) == 0));
     const int v = wide ? V : 1;
-    int tx = 1;
-    while (tx < 256 && (int64_t)tx * v < N) tx *= 2;
+    const int tx = lanes_for(N, v);
     const dim3 grid((unsigned)strips, (unsigned)cdiv(N, (int64_t)tx * v));
     const int64_t rows = cdiv(M, strips);
-    if (wide) hipLaunchKernelGGL((dact_kernel<T, V>), grid, dim3(256), 0, s, (const T *)dy, lddy, (const T *)z, ldz, act, slope, M, N, rows, tx, (T *)dz, part);
-    else hipLaunchKernelGGL((dact_kernel<T, 1>), grid, dim3(256), 0, s, (const T *)dy, lddy, (const T *)z, ldz, act, slope, M, N, rows, tx, (T *)dz, part);
+    if (wide) hipLaunchKernelGGL((dact_kernel<T, V>), grid, dim3(256), 0, s, (const T *)dy, lddy, (const T *)z, ldz, act, slope, M, N, rows, tx, (T *)dz, part, (T *)db);
+    else hipLaunchKernelGGL((dact_kernel<T, 1>), grid, dim3(256), 0, s, (const T *)dy, lddy, (const T *)z, ldz, act, slope, M, N, rows, tx, (T *)dz, part, (T *)db);
     AVC_HIP(hipGetLastError());
     return AVC_OK;
 }
@@ -392,7 +420,7 @@ static BackwardSpace backward_space(int64_t M, int64_t N, int64_t K, int dtype)
 {
     BackwardSpace w;
     w.dz = align256((size_t)M * N * esize(dtype));
-    w.strips = align256(sizeof(float) * (size_t)strips_for(M, N) * N);
+    w.strips = align256(sizeof(float) * (size_t)strips_for(M, N, dtype) * N);
     w.partial = partial_bytes(plan_tiles(N, K, M, dtype), N, K);
     if (M) w.partial = std::max(w.partial, partial_bytes(plan_tiles(M, K, N, dtype), M, K));
     w.total = w.dz + w.strips + w.partial;
@@ -417,10 +445,11 @@ int backward(const void *dy, int64_t lddy, const Operand &x, const void *w, int6
     char *dz_buf = (char *)ws, *strips_buf = dz_buf + sp.dz, *part = strips_buf + sp.strips;
     const bool active = act != AVC_ACT_NONE;
     if (active || db) {
-        const int64_t strips = strips_for(M, N);
-        const int rc = AVC_BY_TYPE(dtype, launch_dact)(dy, lddy, active ? z : nullptr, ldz, act, slope, M, N, dz_buf, db ? (float *)strips_buf : nullptr, strips, s);
+        const int64_t strips = strips_for(M, N, dtype);
+        const int rc = AVC_BY_TYPE(dtype, launch_dact)(dy, lddy, active ? z : nullptr, ldz, act, slope, M, N, dz_buf, db && strips > 1 ? (float *)strips_buf : nullptr,
+                                                       strips == 1 ? db : nullptr, strips, s);
         if (rc != AVC_OK) return rc;
-        if (db) {
+        if (db && strips > 1) {
             const int rc2 = launch_columns((const float *)strips_buf, (int)strips, N, N, dtype, db, nullptr, s);
             if (rc2 != AVC_OK) return rc2;
         }

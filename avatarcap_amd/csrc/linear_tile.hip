@@ -12,6 +12,7 @@
 // float32 runs on the same bf16 matrix instructions: x = h + m + l, three bf16 of 8 significant bits each (rounded to nearest, so the three hold all 24 bits exactly), and
 // x w = hh + (hm + mh) + (hl + mm + lh) + terms below 2^-23 |x w| that float32's own products would round away.  Six products at the bf16 rate are faster than one at the f32
 // matrix rate.  The head is clamped to bf16's largest finite value, so that a value beyond it (and an infinity, which then travels in the tail) does not become inf - inf.
+#include <atomic>
 #include <type_traits>
 #include "avcap_internal.h"
 #include "linear.h"
@@ -460,7 +461,16 @@ template <int BM, int BN, int WM, int WN, bool PKC, bool QKC, bool DMA> int laun
     constexpr int LDS = stages(BM) * NP * (Tile<BM, PKC>::BYTES + Tile<BN, QKC>::BYTES);
     static_assert(LDS <= 160 * 1024, "tile does not fit LDS");
     auto k = tile_kernel<BM, BN, WM, WN, PKC, QKC, DMA>;
-    if (LDS > 64 * 1024) AVC_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+    if (LDS > 64 * 1024) {                                              // once per device
+        static std::atomic<uint64_t> allowed{0};
+        int device = 0;
+        AVC_HIP(hipGetDevice(&device));
+        const uint64_t bit = 1ull << (device & 63);
+        if (device > 63 || !(allowed.load(std::memory_order_acquire) & bit)) {
+            AVC_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+            allowed.fetch_or(bit, std::memory_order_release);
+        }
+    }
     hipLaunchKernelGGL(k, dim3((unsigned)((int64_t)a.tiles_m * a.tiles_n * a.splits)), dim3(WM * WN * 64), LDS, s, a);
     AVC_HIP(hipGetLastError());
     return AVC_OK;

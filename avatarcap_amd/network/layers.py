@@ -11,6 +11,7 @@ No gradient of a gradient.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -65,23 +66,48 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _space(nbytes, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+# Bytes of workspace, a function of sizes and type alone.
+@functools.lru_cache(maxsize=4096)
+def _forward_bytes(m, n, k, dt, xr, xc):
+    nbytes = C.c_int64()
+    _lib.check(_lib.lib().avc_linear_workspace(m, n, k, dt, xr, xc, C.byref(nbytes)))
+    return nbytes.value
+
+
+@functools.lru_cache(maxsize=4096)
+def _backward_bytes(m, n, k, dt):
+    nbytes = C.c_int64()
+    _lib.check(_lib.lib().avc_linear_backward_workspace(m, n, k, dt, C.byref(nbytes)))
+    return nbytes.value
+
+
+@functools.lru_cache(maxsize=4096)
+def _norm_backward_bytes(m, c, dt):
+    nbytes = C.c_int64()
+    _lib.check(_lib.lib().avc_layer_norm_backward_workspace(m, c, dt, C.byref(nbytes)))
+    return nbytes.value
+
+
+def _space(nbytes, like):
+    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+
+
+def _stream(t):
+    return torch.cuda.current_stream(t.device).cuda_stream
 
 
 def _linear_forward(x, w, bias, res, act, slope, want_z):
     m, k = x.shape
     n = w.shape[0]
-    L, dev, dt = _lib.lib(), x.device, DTYPES[x.dtype]
+    dt = DTYPES[x.dtype]
     x, xr, xc = _matrix(x)
     w = _rows(w)
-    y = torch.empty((m, n), dtype=x.dtype, device=dev)
-    z = torch.empty_like(y) if want_z else None
-    nbytes = C.c_int64()
-    _lib.check(L.avc_linear_workspace(m, n, k, dt, xr, xc, C.byref(nbytes)))
-    ws = _space(nbytes.value, dev)
-    _lib.check(L.avc_linear(_lib.ctx(dev), x.data_ptr(), xr, xc, w.data_ptr(), _row_stride(w), _ptr(bias), _ptr(res), 0 if res is None else _row_stride(res), act, slope, m, n, k, dt,
-                            y.data_ptr(), n, _ptr(z), n, _ptr(ws), nbytes.value, _lib.stream_ptr(dev)))
+    y = x.new_empty((m, n))
+    z = x.new_empty((m, n)) if want_z else None
+    nbytes = _forward_bytes(m, n, k, dt, xr, xc)
+    ws = _space(nbytes, x)
+    _lib.check(_lib.lib().avc_linear(_lib.ctx(x.device), x.data_ptr(), xr, xc, w.data_ptr(), _row_stride(w), _ptr(bias), _ptr(res), 0 if res is None else _row_stride(res), act, slope, m, n, k,
+                                     dt, y.data_ptr(), n, _ptr(z), n, _ptr(ws), nbytes, _stream(x)))
     return y, z
 
 
@@ -100,25 +126,19 @@ class _Linear(torch.autograd.Function):
     def backward(ctx, dy):
         x, w, saved = ctx.saved_tensors
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        (m, k), n = x.shape, w.shape[0]
-        dev, dt = dy.device, DTYPES[dy.dtype]
         dx = dw = db = None
         if need_x or need_w or need_b:
-            L = _lib.lib()
+            (m, k), n, dt = x.shape, w.shape[0], DTYPES[dy.dtype]
             g = _rows(dy)
             x, xr, xc = _matrix(x)
             w = _rows(w)
-            if need_x:
-                dx = torch.empty((m, k), dtype=dy.dtype, device=dev)
-            if need_w:
-                dw = torch.empty((n, k), dtype=dy.dtype, device=dev)
-            if need_b:
-                db = torch.empty((n,), dtype=dy.dtype, device=dev)
-            nbytes = C.c_int64()
-            _lib.check(L.avc_linear_backward_workspace(m, n, k, dt, C.byref(nbytes)))
-            ws = _space(nbytes.value, dev)
-            _lib.check(L.avc_linear_backward(_lib.ctx(dev), g.data_ptr(), _row_stride(g), x.data_ptr(), xr, xc, w.data_ptr(), _row_stride(w), _ptr(saved), n, ctx.act, ctx.slope, m, n, k, dt,
-                                             _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes.value, _lib.stream_ptr(dev)))
+            dx = g.new_empty((m, k)) if need_x else None
+            dw = g.new_empty((n, k)) if need_w else None
+            db = g.new_empty((n,)) if need_b else None
+            nbytes = _backward_bytes(m, n, k, dt)
+            ws = _space(nbytes, g)
+            _lib.check(_lib.lib().avc_linear_backward(_lib.ctx(g.device), g.data_ptr(), _row_stride(g), x.data_ptr(), xr, xc, w.data_ptr(), _row_stride(w), _ptr(saved), n, ctx.act, ctx.slope,
+                                                      m, n, k, dt, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes, _stream(g)))
         return dx, dw, db, dy if need_r else None, None, None
 
 
@@ -159,13 +179,11 @@ def linear(x, weight, bias=None, act=None, slope=0.02, residual=None):
 
 def _norm_forward(x, g, b, eps, want_stats):
     m, c = x.shape
-    dev = x.device
     x = _rows(x)
-    y = torch.empty((m, c), dtype=x.dtype, device=dev)
-    stats = torch.empty((2, m), dtype=torch.float32, device=dev) if want_stats else None
+    y = x.new_empty((m, c))
+    stats = x.new_empty((2, m), dtype=torch.float32) if want_stats else None
     p = _ptr(stats)
-    _lib.check(_lib.lib().avc_layer_norm(_lib.ctx(dev), x.data_ptr(), _row_stride(x), _ptr(g), _ptr(b), eps, m, c, DTYPES[x.dtype], y.data_ptr(), c, p, p + 4 * m if p else p,
-                                         _lib.stream_ptr(dev)))
+    _lib.check(_lib.lib().avc_layer_norm(_lib.ctx(x.device), x.data_ptr(), _row_stride(x), _ptr(g), _ptr(b), eps, m, c, DTYPES[x.dtype], y.data_ptr(), c, p, p + 4 * m if p else p, _stream(x)))
     return y, stats
 
 
@@ -181,19 +199,16 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, dy):
         x, g, stats = ctx.saved_tensors
         need_x, need_g, need_b = ctx.needs_input_grad[:3]
-        m, c = x.shape
-        L, dev, dt = _lib.lib(), dy.device, DTYPES[dy.dtype]
+        (m, c), dt = x.shape, DTYPES[dy.dtype]
         x, dy = _rows(x), _rows(dy)
-        dx = torch.empty((m, c), dtype=dy.dtype, device=dev) if need_x else None
-        dg = torch.empty((c,), dtype=dy.dtype, device=dev) if need_g else None
-        db = torch.empty((c,), dtype=dy.dtype, device=dev) if need_b else None
-        nbytes = C.c_int64()
-        if need_g or need_b:
-            _lib.check(L.avc_layer_norm_backward_workspace(m, c, dt, C.byref(nbytes)))
-        ws = _space(nbytes.value, dev)
+        dx = dy.new_empty((m, c)) if need_x else None
+        dg = dy.new_empty((c,)) if need_g else None
+        db = dy.new_empty((c,)) if need_b else None
+        nbytes = _norm_backward_bytes(m, c, dt) if need_g or need_b else 0
+        ws = _space(nbytes, dy)
         p = stats.data_ptr()
-        _lib.check(L.avc_layer_norm_backward(_lib.ctx(dev), dy.data_ptr(), _row_stride(dy), x.data_ptr(), _row_stride(x), _ptr(g), p, p + 4 * m, m, c, dt, _ptr(dx), c, _ptr(dg), _ptr(db),
-                                             _ptr(ws), nbytes.value, _lib.stream_ptr(dev)))
+        _lib.check(_lib.lib().avc_layer_norm_backward(_lib.ctx(dy.device), dy.data_ptr(), _row_stride(dy), x.data_ptr(), _row_stride(x), _ptr(g), p, p + 4 * m, m, c, dt, _ptr(dx), c, _ptr(dg),
+                                                      _ptr(db), _ptr(ws), nbytes, _stream(dy)))
         return dx, dg, db, None
 
 
