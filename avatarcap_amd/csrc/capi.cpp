@@ -411,7 +411,7 @@ int avc_layer_norm_backward(avc_ctx *ctx, const void *dy, int64_t lddy, const vo
     AVC_REQUIRE(ctx && (!M || (dy && x && mean && rstd)), AVC_ERR_ARG, "avc_layer_norm_backward: NULL argument");
     AVC_REQUIRE(ldx >= 0 && lddy >= 0 && (!dx || lddx >= C), AVC_ERR_ARG, "avc_layer_norm_backward: a row stride is negative or lddx shorter than the row");
     if (dgamma || dbeta)
-        AVC_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= (int64_t)lin::layer_norm_backward_workspace(M, C, dtype), AVC_ERR_CAPACITY,
+        AVC_REQUIRE(((uintptr_t)workspace & 15) == 0 && workspace_bytes >= (int64_t)lin::layer_norm_backward_workspace(M, C, dtype) && (workspace || !workspace_bytes), AVC_ERR_CAPACITY,
                     "avc_layer_norm_backward: needs %lld bytes of 16-byte aligned workspace, got %lld", (long long)lin::layer_norm_backward_workspace(M, C, dtype), (long long)workspace_bytes);
     AVC_ON_DEVICE(ctx);
     return lin::layer_norm_backward(dy, lddy, x, ldx, gamma, mean, rstd, M, C, dtype, dx, lddx, dgamma, dbeta, (float *)workspace, (hipStream_t)stream);

@@ -218,7 +218,7 @@ __global__ __launch_bounds__(TPR ? TPR : 256) void norm_backward_kernel(const T 
             store_run<V>(dx + m * lddx, Run<V>(((int64_t)c * tpr + lane) * V, C), t[c]);
         }
     }
-    if (!part) return;
+    if (!dg_out && !db_out) return;
     float *out = part + (int64_t)blockIdx.x * 2 * C;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
@@ -362,7 +362,8 @@ template <typename T> int norm_backward(const void *dy, int64_t lddy, const void
 {
     const Spread sp = spread_of(C, dtype);
     const int64_t blocks = backward_blocks(M, C, dtype);
-    float *p = dg || db ? part : nullptr;
+    const bool sums = dg || db;
+    float *p = part;
     constexpr int W = Width<T>::V;
 #define AVC_NORM(V, TPR, NCH, BLOCK)                                                                                                                                \
     hipLaunchKernelGGL((norm_backward_kernel<T, V, TPR, NCH>), dim3((unsigned)blocks), dim3(BLOCK), 0, s, (const T *)dy, lddy, (const T *)x, ldx, (const T *)g, mean, rstd, M, C, sp.tpr_log,       \
@@ -370,7 +371,7 @@ template <typename T> int norm_backward(const void *dy, int64_t lddy, const void
     if (sp.narrow) AVC_NORM(1, 0, 1, 256);
     else if (sp.tpr == 0) {
         if (dx && M) hipLaunchKernelGGL(norm_backward_long_kernel<T>, dim3((unsigned)std::min<int64_t>(M, MAX_GRID)), dim3(1024), 0, s, (const T *)dy, lddy, (const T *)x, ldx, (const T *)g, mean, rstd, M, C, (T *)dx, lddx);
-        if (p)
+        if (sums)
             hipLaunchKernelGGL(norm_columns_kernel<T>, dim3((unsigned)blocks, (unsigned)cdiv(C, 256 * Width<T>::V)), dim3(256), 0, s, (const T *)dy, lddy, (const T *)x, ldx, mean, rstd, M, C,
                                cdiv(M, blocks), p);
     } else if (sp.tpr <= 64) {
@@ -380,7 +381,7 @@ template <typename T> int norm_backward(const void *dy, int64_t lddy, const void
     } else AVC_NORM(W, 1024, 2, 1024);
 #undef AVC_NORM
     AVC_HIP(hipGetLastError());
-    if (p && (blocks > 1 || sp.tpr == 0)) return launch_colsum2(p, (int)blocks, C, dtype, dg, db, s);
+    if (sums && (blocks > 1 || sp.tpr == 0)) return launch_colsum2(p, (int)blocks, C, dtype, dg, db, s);
     return AVC_OK;
 }
 
@@ -393,7 +394,11 @@ int layer_norm(const void *x, int64_t ldx, const void *g, const void *b, float e
     return norm_forward<_Float16>(x, ldx, g, b, eps, M, C, dtype, y, ldy, mean, rstd, s);
 }
 
-size_t layer_norm_backward_workspace(int64_t M, int64_t C, int dtype) { return sizeof(float) * 2 * (size_t)backward_blocks(M, C, dtype) * (size_t)C; }
+size_t layer_norm_backward_workspace(int64_t M, int64_t C, int dtype)
+{
+    const int64_t blocks = backward_blocks(M, C, dtype);
+    return blocks == 1 && spread_of(C, dtype).tpr ? 0 : sizeof(float) * 2 * (size_t)blocks * (size_t)C;   // a single workgroup writes the gradients itself
+}
 
 int layer_norm_backward(const void *dy, int64_t lddy, const void *x, int64_t ldx, const void *g, const float *mean, const float *rstd, int64_t M, int64_t C, int dtype, void *dx, int64_t lddx,
                         void *dg, void *db, float *part, hipStream_t s)

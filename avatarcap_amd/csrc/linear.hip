@@ -91,17 +91,22 @@ template <typename T, int FB> __global__ __launch_bounds__(1024) void few_kernel
     f32x4 acc[FB];
 #pragma unroll
     for (int b = 0; b < FB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
-    constexpr int CK = Chunk<T>::K, U = 4;
+    constexpr int CK = Chunk<T>::K, U = 4 / FB;
     const int64_t stride = (int64_t)a.kw * CK, qk = q * Chunk<T>::LANE;
     int64_t k = (int64_t)kslot * CK;
-    for (; k + (U - 1) * stride + CK <= a.K; k += U * stride) {
-        Chunk<T> s[U];
+    for (; k + (U - 1) * stride + CK <= a.K; k += U * stride) {        // U chunks of both operands on their way before the first is used
+        Chunk<T> s[U], f[U][FB];
 #pragma unroll
-        for (int u = 0; u < U; ++u) s[u] = load_chunk(srow, k + u * stride + qk);
+        for (int u = 0; u < U; ++u) {
+            s[u] = load_chunk(srow, k + u * stride + qk);
+#pragma unroll
+            for (int b = 0; b < FB; ++b) f[u][b] = load_chunk(frow[b], k + u * stride + qk);
+        }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int b = 0; b < FB; ++b) acc[b] = chunk_mfma(s[u], load_chunk(frow[b], k + u * stride + qk), acc[b]);
+            for (int b = 0; b < FB; ++b) acc[b] = chunk_mfma(s[u], f[u][b], acc[b]);
     }
     for (; k + CK <= a.K; k += stride) {
         const Chunk<T> s = load_chunk(srow, k + qk);
@@ -282,6 +287,7 @@ int launch_colsum2(const float *part, int strips, int64_t C, int dtype, void *ou
 namespace {
 
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline int esize(int dtype) { return dtype == AVC_F32 ? 4 : 2; }
 
 // ---- which tile, how many splits: from the sizes alone, so that the workspace can be asked for in advance -----------------------------------------------------------
 // The time of a launch is estimated for every tile shape and a ladder of splits, and the least taken.  With W workgroups on the fullest CU, `occ` of them at a time, and S steps of
@@ -293,7 +299,7 @@ constexpr TileCost COST_16[3] = {{1, 1.62, 7.0, 0.01, 11.1}, {2, 0.91, 1.9, 0.47
 constexpr TileCost COST_F32[3] = {{1, 2.67, 5.4, 0.00, 12.0}, {3, 3.64, 1.7, 1.57, 4.3}, {3, 0.89, 1.7, 0.57, 1.0}};
 constexpr int SPLITS[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256};
 
-struct Plan { int tile, tiles_m, tiles_n, splits; int64_t kper; };
+struct Plan { int tile, tiles_m, tiles_n, splits; int64_t kper; double us; };
 
 Plan plan_tiles(int64_t M, int64_t N, int64_t K, int dtype)
 {
@@ -311,7 +317,7 @@ Plan plan_tiles(int64_t M, int64_t N, int64_t K, int dtype)
             if (splits > 1) us += 3 + 8e-6 / 5 * (double)splits * M * N;
             if (!best.splits || us < least) {
                 least = us;
-                best = Plan{tile, (int)tm, (int)tn, (int)splits, kper};
+                best = Plan{tile, (int)tm, (int)tn, (int)splits, kper, us};
             }
         }
     }
@@ -319,7 +325,24 @@ Plan plan_tiles(int64_t M, int64_t N, int64_t K, int dtype)
 }
 size_t partial_bytes(const Plan &p, int64_t M, int64_t N) { return p.splits > 1 ? sizeof(float) * (size_t)p.splits * (size_t)M * (size_t)N : 0; }
 
-inline int esize(int dtype) { return dtype == AVC_F32 ? 4 : 2; }
+// Large products whose last round of the large tile is mostly empty are cut: `rows` rows in full rounds, the rest in a launch of its own with the tile that suits it.  65537 rows of
+// 545 -> 256 float32 values need 514 tiles, three rounds of 256 for two rounds' work: 176 us; cut at 65536, 124 us.
+struct Cut { int64_t rows; Plan main, rest; };
+Cut plan_cut(int64_t M, int64_t N, int64_t K, int dtype)
+{
+    Cut c{M, plan_tiles(M, N, K, dtype), Plan{}};
+    const int bm = tile_bm(dtype, TILE_BIG);
+    const int64_t tn = cdiv(N, tile_bn(dtype, TILE_BIG)), rounds = cdiv(M, bm) * tn / 256, rows = rounds * 256 / tn * bm;
+    if (rounds < 1 || rounds > 16 || rows < 1 || rows >= M || c.main.splits > 1) return c;
+    const Plan main = plan_tiles(rows, N, K, dtype), rest = plan_tiles(M - rows, N, K, dtype);
+    if (main.splits == 1 && main.us + rest.us + 3 < c.main.us) return Cut{rows, main, rest};
+    return c;
+}
+size_t product_bytes(int64_t M, int64_t N, int64_t K, int dtype)
+{
+    const Cut c = plan_cut(M, N, K, dtype);
+    return std::max(partial_bytes(c.main, c.rows, N), c.rows < M ? partial_bytes(c.rest, M - c.rows, N) : 0);
+}
 
 // lanes that share a row in the activation-gradient pass
 int lanes_for(int64_t N, int v)
@@ -344,9 +367,8 @@ template <typename T> int launch_reduce(const float *part, int splits, int64_t M
     return AVC_OK;
 }
 
-int product(const Operand &P, const Operand &Q, int64_t M, int64_t N, int64_t K, int dtype, const Epilogue &e, void *out, int64_t ldo, void *ws, hipStream_t s)
+int product_rows(const Operand &P, const Operand &Q, int64_t M, int64_t N, int64_t K, int dtype, const Epilogue &e, void *out, int64_t ldo, void *ws, const Plan &p, hipStream_t s)
 {
-    const Plan p = plan_tiles(M, N, K, dtype);
     AVC_REQUIRE((int64_t)p.tiles_m * p.tiles_n * p.splits < (1 << 22), AVC_ERR_ARG, "avc_linear: %lld x %lld outputs are more than one launch covers", (long long)M, (long long)N);
     TileArgs a{P, Q, M, N, K, out, ldo, e, (float *)ws, p.kper, p.tiles_m, p.tiles_n, p.splits};
     const int rc = dtype == AVC_F32 ? launch_tile_f32(a, p.tile, s) : dtype == AVC_BF16 ? launch_tile_bf16(a, p.tile, s) : launch_tile_f16(a, p.tile, s);
@@ -354,6 +376,21 @@ int product(const Operand &P, const Operand &Q, int64_t M, int64_t N, int64_t K,
     if (dtype == AVC_F32) return launch_reduce<float>(a.partial, p.splits, M, N, out, ldo, e, s);
     if (dtype == AVC_BF16) return launch_reduce<__bf16>(a.partial, p.splits, M, N, out, ldo, e, s);
     return launch_reduce<_Float16>(a.partial, p.splits, M, N, out, ldo, e, s);
+}
+
+inline const void *ahead(const void *p, int64_t elements, int dtype) { return p ? (const char *)p + elements * esize(dtype) : nullptr; }
+
+int product(const Operand &P, const Operand &Q, int64_t M, int64_t N, int64_t K, int dtype, const Epilogue &e, void *out, int64_t ldo, void *ws, hipStream_t s)
+{
+    const Cut c = plan_cut(M, N, K, dtype);
+    if (c.rows < M) {                                                    // the rows past the full rounds
+        const int64_t m = c.rows;
+        const Operand below{ahead(P.p, P.kc ? m * P.ld : m, dtype), P.ld, P.kc};
+        const Epilogue eb{e.bias, ahead(e.res, m * e.ldr, dtype), e.ldr, (void *)ahead(e.z, m * e.ldz, dtype), e.ldz, e.act, e.slope};
+        const int rc = product_rows(below, Q, M - m, N, K, dtype, eb, (void *)ahead(out, m * ldo, dtype), ldo, ws, c.rest, s);
+        if (rc != AVC_OK) return rc;
+    }
+    return product_rows(P, Q, c.rows, N, K, dtype, e, out, ldo, ws, c.main, s);
 }
 
 // ---- few rows ----------------------------------------------------------------------------------------------------------------------------------------------------
@@ -412,7 +449,7 @@ template <typename T> int launch_dact(const void *dy, int64_t lddy, const void *
 
 size_t forward_workspace(int64_t M, int64_t N, int64_t K, int dtype, bool x_kc)
 {
-    return M && route(M, N, x_kc) == ROUTE_TILE ? partial_bytes(plan_tiles(M, N, K, dtype), M, N) : 0;
+    return M && route(M, N, x_kc) == ROUTE_TILE ? product_bytes(M, N, K, dtype) : 0;
 }
 
 struct BackwardSpace { size_t dz, strips, partial, total; };
@@ -421,8 +458,8 @@ static BackwardSpace backward_space(int64_t M, int64_t N, int64_t K, int dtype)
     BackwardSpace w;
     w.dz = align256((size_t)M * N * esize(dtype));
     w.strips = align256(sizeof(float) * (size_t)strips_for(M, N, dtype) * N);
-    w.partial = partial_bytes(plan_tiles(N, K, M, dtype), N, K);
-    if (M) w.partial = std::max(w.partial, partial_bytes(plan_tiles(M, K, N, dtype), M, K));
+    w.partial = product_bytes(N, K, M, dtype);
+    if (M) w.partial = std::max(w.partial, product_bytes(M, K, N, dtype));
     w.total = w.dz + w.strips + w.partial;
     return w;
 }

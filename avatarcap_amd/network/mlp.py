@@ -1,12 +1,15 @@
 """Parameter containers with the reference's state_dict surface for `network/mlp.py`.
 
-These modules hold weights only (so `load_state_dict(torch.load(...)['network'])` works with the
-reference's checkpoints).  They deliberately have NO forward(): the math runs
-in the fused HIP kernels (csrc/fused_mlp.hip) after `pack` folds BatchNorm / weight_norm; there is
-no eager fallback to route to by accident.
+The modules carry the reference's keys (so `load_state_dict(torch.load(...)['network'])` works with
+its checkpoints).  The networks' queries do not call them: their math runs in the fused HIP kernels
+(csrc/fused_mlp.hip) after `pack` folds BatchNorm / weight_norm.  `MLP.forward` runs a stack of any
+widths layer by layer on the dense-layer kernels (network/layers.py), with gradients; there is no CPU
+path.  `OffsetDecoder` holds weights only.
 """
 import torch
 import torch.nn as nn
+
+from .layers import linear
 
 
 def _conv1(cin, cout):
@@ -35,8 +38,27 @@ class MLP(nn.Module):
             self.fc_list.append(nn.Sequential(conv, nn.Identity()))
         self.fc_list.append(_conv1(self.all_channels[-2], out_channels))
 
-    def forward(self, *a, **k):
-        raise RuntimeError('avatarcap_amd MLP is a weight container; queries run in the HIP library')
+    @staticmethod
+    def _weight(conv):
+        """The layer's (cout, cin) weight; g v / ||v|| per output where it is weight-normed."""
+        w = torch._weight_norm(conv.weight_v, conv.weight_g, 0) if hasattr(conv, 'weight_g') else conv.weight
+        return w[:, :, 0]
+
+    def forward(self, x):
+        """x (B, in_channels, N) -> (B, out_channels, N)   (mlp.py:56-72): x <- act(W_l [x | x0 if l in res_layers] + b_l), the last layer without an activation but for `last_op`.
+        float32, bfloat16 or float16, input and weights alike, on the HIP device.  Differentiable in x and the parameters."""
+        if x.dim() != 3 or x.shape[1] != self.all_channels[0]:
+            raise ValueError(f'MLP: expected (B, {self.all_channels[0]}, N), got {tuple(x.shape)}')
+        B, _, N = x.shape
+        x0 = x[0].t() if B == 1 else x.transpose(1, 2).reshape(B * N, -1)      # points as rows; for one batch entry a view that the kernels read as it lies
+        h = x0
+        last = len(self.fc_list) - 1
+        for l, fc in enumerate(self.fc_list):
+            conv = fc if l == last else fc[0]
+            if l in self.res_layers:
+                h = torch.cat([h, x0], dim=1)
+            h = linear(h, self._weight(conv), conv.bias, act=self.last_op if l == last else self.nlactv)
+        return h.reshape(B, N, -1).transpose(1, 2).contiguous()
 
 
 class OffsetDecoder(nn.Module):
