@@ -370,7 +370,7 @@ int avc_linear_backward(avc_ctx *ctx, const void *dy, int64_t lddy, const void *
     if (dw)
         if (int rc = check_x("avc_linear_backward", x_row, x_col, M, K)) return rc;
     AVC_REQUIRE(lddy >= 0 && ldw >= 0 && (act == AVC_ACT_NONE || ld_saved >= 0), AVC_ERR_ARG, "avc_linear_backward: a row stride is negative");
-    AVC_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= (int64_t)lin::backward_workspace(M, N, K, dtype), AVC_ERR_CAPACITY,
+    AVC_REQUIRE(((uintptr_t)workspace & 15) == 0 && workspace_bytes >= (int64_t)lin::backward_workspace(M, N, K, dtype) && (workspace || !workspace_bytes), AVC_ERR_CAPACITY,
                 "avc_linear_backward: needs %lld bytes of 16-byte aligned workspace, got %lld", (long long)lin::backward_workspace(M, N, K, dtype), (long long)workspace_bytes);
     AVC_ON_DEVICE(ctx);
     return lin::backward(dy, lddy, x_operand(x, x_row, x_col), w, ldw, saved, ld_saved, act, slope, M, N, K, dtype, dx, dw, db, workspace, (hipStream_t)stream);

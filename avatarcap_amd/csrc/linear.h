@@ -45,6 +45,19 @@ inline int tile_bm(int dtype, int tile) { return tile == TILE_BIG ? 256 : tile =
 inline int tile_bn(int dtype, int tile) { return tile == TILE_BIG ? (dtype == AVC_F32 ? 128 : 256) : tile == TILE_MID ? 128 : 64; }
 inline int tile_bk(int dtype) { return dtype == AVC_F32 ? 32 : 64; }
 
+// the backward pass of a small layer in one launch: products of 64 x 64 tiles without splits (P of both is dy), and the column sums; tiles_m = 0 or db = NULL: not asked for
+struct SmallArgs {
+    TileArgs dx, dw;
+    const void *dy; int64_t lddy;
+    const void *saved; int64_t ld_saved;
+    int act; float slope;
+    int64_t M, N;
+    void *db;
+};
+int launch_small_f32(const SmallArgs &a, unsigned blocks, bool x_kc, hipStream_t s);
+int launch_small_bf16(const SmallArgs &a, unsigned blocks, bool x_kc, hipStream_t s);
+int launch_small_f16(const SmallArgs &a, unsigned blocks, bool x_kc, hipStream_t s);
+
 int launch_tile_f32(const TileArgs &a, int tile, hipStream_t s);
 int launch_tile_bf16(const TileArgs &a, int tile, hipStream_t s);
 int launch_tile_f16(const TileArgs &a, int tile, hipStream_t s);

@@ -129,13 +129,27 @@ template <typename T, int FB> __global__ __launch_bounds__(1024) void few_kernel
     }
 #pragma unroll
     for (int b = 0; b < FB; ++b) {
-        const int f = 16 * b + l16;
-        if (f >= a.nf) continue;
+        const int f = min(16 * b + l16, a.nf - 1);
+        float bias[4], res[4], v[4];
+        int64_t m[4], n[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t s = s0 + 4 * q + j;
-            if (s < a.ns) finish<T>(acc[b][j], a.rows_are_f ? f : s, a.rows_are_f ? s : f, a.ep, a.out, a.ldo);
+        for (int j = 0; j < 4; ++j) {                                   // every load before the first store: the outputs may lie on the residual
+            const int64_t s = min(s0 + 4 * q + j, a.ns - 1);
+            m[j] = a.rows_are_f ? f : s;
+            n[j] = a.rows_are_f ? s : f;
+            bias[j] = a.ep.bias ? (float)((const T *)a.ep.bias)[n[j]] : 0.f;
+            res[j] = a.ep.res ? (float)((const T *)a.ep.res)[m[j] * a.ep.ldr + n[j]] : 0.f;
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = acc[b][j] + bias[j];
+        const bool mine = 16 * b + l16 < a.nf;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (a.ep.z && mine && s0 + 4 * q + j < a.ns) ((T *)a.ep.z)[m[j] * a.ep.ldz + n[j]] = (T)v[j];
+        act_run<4>(v, a.ep.act, a.ep.slope);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (mine && s0 + 4 * q + j < a.ns) a.out[m[j] * a.ldo + n[j]] = (T)(a.ep.res ? v[j] + res[j] : v[j]);
     }
 }
 
@@ -326,7 +340,7 @@ Plan plan_tiles(int64_t M, int64_t N, int64_t K, int dtype)
 size_t partial_bytes(const Plan &p, int64_t M, int64_t N) { return p.splits > 1 ? sizeof(float) * (size_t)p.splits * (size_t)M * (size_t)N : 0; }
 
 // Large products whose last round of the large tile is mostly empty are cut: `rows` rows in full rounds, the rest in a launch of its own with the tile that suits it.  65537 rows of
-// 545 -> 256 float32 values need 514 tiles, three rounds of 256 for two rounds' work: 176 us; cut at 65536, 124 us.
+// 545 -> 256 float32 values need 514 tiles, three rounds of 256 for two rounds' work: 171 us; cut at 65536, 133 us.
 struct Cut { int64_t rows; Plan main, rest; };
 Cut plan_cut(int64_t M, int64_t N, int64_t K, int dtype)
 {
@@ -452,10 +466,18 @@ size_t forward_workspace(int64_t M, int64_t N, int64_t K, int dtype, bool x_kc)
     return M && route(M, N, x_kc) == ROUTE_TILE ? product_bytes(M, N, K, dtype) : 0;
 }
 
+// Layers whose gradients are a few dozen tiles with short sums: the launches would cost more than the work, so one launch does it all (no workspace).  17 x 33 -> 65 with a bias:
+// one launch instead of three.
+static bool small_backward(int64_t M, int64_t N, int64_t K)
+{
+    return M >= 1 && M <= 512 && N <= 1024 && cdiv(N, 64) * cdiv(K, 64) <= 256 && cdiv(M, 64) * cdiv(K, 64) <= 256;
+}
+
 struct BackwardSpace { size_t dz, strips, partial, total; };
 static BackwardSpace backward_space(int64_t M, int64_t N, int64_t K, int dtype)
 {
-    BackwardSpace w;
+    BackwardSpace w{};
+    if (small_backward(M, N, K)) return w;
     w.dz = align256((size_t)M * N * esize(dtype));
     w.strips = align256(sizeof(float) * (size_t)strips_for(M, N, dtype) * N);
     w.partial = product_bytes(N, K, M, dtype);
@@ -478,6 +500,19 @@ int forward(const Operand &x, const void *w, int64_t ldw, int64_t M, int64_t N, 
 int backward(const void *dy, int64_t lddy, const Operand &x, const void *w, int64_t ldw, const void *z, int64_t ldz, int act, float slope, int64_t M, int64_t N, int64_t K, int dtype,
              void *dx, void *dw, void *db, void *ws, hipStream_t s)
 {
+    const Epilogue none{nullptr, nullptr, 0, nullptr, 0, AVC_ACT_NONE, 0.f};
+    if (small_backward(M, N, K)) {
+        SmallArgs a{};
+        auto tiles = [](TileArgs &t, const Operand &P, const Operand &Q, int64_t m, int64_t n, int64_t k, void *out) {
+            t = TileArgs{P, Q, m, n, k, out, n, Epilogue{nullptr, nullptr, 0, nullptr, 0, AVC_ACT_NONE, 0.f}, nullptr, k, (int)cdiv(m, 64), (int)cdiv(n, 64), 1};
+        };
+        if (dx) tiles(a.dx, Operand{dy, lddy, 1}, Operand{w, ldw, 0}, M, K, N, dx);
+        if (dw) tiles(a.dw, Operand{dy, lddy, 0}, Operand{x.p, x.ld, x.kc ? 0 : 1}, N, K, M, dw);
+        a.dy = dy; a.lddy = lddy; a.saved = z; a.ld_saved = ldz; a.act = act; a.slope = slope; a.M = M; a.N = N; a.db = db;
+        const int64_t blocks = (int64_t)a.dx.tiles_m * a.dx.tiles_n + (int64_t)a.dw.tiles_m * a.dw.tiles_n + (db ? cdiv(N, 16) : 0);
+        if (!blocks) return AVC_OK;
+        return dtype == AVC_F32 ? launch_small_f32(a, (unsigned)blocks, x.kc, s) : dtype == AVC_BF16 ? launch_small_bf16(a, (unsigned)blocks, x.kc, s) : launch_small_f16(a, (unsigned)blocks, x.kc, s);
+    }
     const BackwardSpace sp = backward_space(M, N, K, dtype);
     char *dz_buf = (char *)ws, *strips_buf = dz_buf + sp.dz, *part = strips_buf + sp.strips;
     const bool active = act != AVC_ACT_NONE;
@@ -493,7 +528,6 @@ int backward(const void *dy, int64_t lddy, const Operand &x, const void *w, int6
     }
     const void *dz = active ? dz_buf : dy;
     const int64_t lddz = active ? N : lddy;
-    const Epilogue none{nullptr, nullptr, 0, nullptr, 0, AVC_ACT_NONE, 0.f};
     if (dx && M) {
         const int rc = product(Operand{dz, lddz, 1}, Operand{w, ldw, 0}, M, K, N, dtype, none, dx, K, part, s);
         if (rc != AVC_OK) return rc;

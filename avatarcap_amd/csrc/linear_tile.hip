@@ -22,12 +22,15 @@ namespace avc { namespace lin {
 #if defined(AVC_LIN_F32)
 typedef float elem_t;
 #define AVC_LAUNCH launch_tile_f32
+#define AVC_LAUNCH_SMALL launch_small_f32
 #elif defined(AVC_LIN_F16)
 typedef _Float16 elem_t;
 #define AVC_LAUNCH launch_tile_f16
+#define AVC_LAUNCH_SMALL launch_small_f16
 #else
 typedef __bf16 elem_t;
 #define AVC_LAUNCH launch_tile_bf16
+#define AVC_LAUNCH_SMALL launch_small_bf16
 #endif
 
 namespace {
@@ -137,13 +140,13 @@ template <int BR, bool KC, int NW> struct Direct {
 };
 
 // (b) through registers: any alignment, any row length; float32 is split into its three planes on the way into LDS.
-__device__ __forceinline__ void split3(const f32x8 &x, bf16x8 out[3])
+template <typename X> __device__ __forceinline__ void split3(const X &x, bf16x8 out[3])                  // X: f32x8
 {
     constexpr float TOP = 3.3895313892515355e38f;                       // bf16's largest finite value
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const __bf16 h = (__bf16)__builtin_amdgcn_fmed3f(x[j], -TOP, TOP);
-        const float r = x[j] - (float)h;
+        const __bf16 h = (__bf16)__builtin_amdgcn_fmed3f((float)x[j], -TOP, TOP);
+        const float r = (float)x[j] - (float)h;
         const __bf16 m = (__bf16)__builtin_amdgcn_fmed3f(r, -TOP, TOP);
         out[0][j] = h;
         out[1][j] = m;
@@ -193,21 +196,58 @@ template <int BR, bool KC, int NT> struct Staged {
         }
         base += KC ? (int64_t)BK : BK * ld;
     }
+    __device__ static __forceinline__ void put(char *lds, int id, const elem8 &x)
+    {
+        if (!FULL && id >= L::BYTES / 16) return;
+        char *dst = lds + L::at(id / L::PIECES, id % L::PIECES);
+        if constexpr (IS_F32) {
+            bf16x8 s[3];
+            split3(x, s);
+#pragma unroll
+            for (int k = 0; k < 3; ++k) *reinterpret_cast<bf16x8 *>(dst + k * L::BYTES) = s[k];
+        } else {
+            *reinterpret_cast<elem8 *>(dst) = x;
+        }
+    }
     __device__ __forceinline__ void store(char *lds, int tid) const
     {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int id = i * NT + tid, r = id / L::PIECES, p = id % L::PIECES;
-            if (!FULL && id >= L::BYTES / 16) continue;
-            char *dst = lds + L::at(r, p);
-            if constexpr (IS_F32) {
-                bf16x8 s[3];
-                split3(v[i], s);
+        for (int i = 0; i < N; ++i) put(lds, i * NT + tid, v[i]);
+    }
+};
+
+// the same for dz = dy act'(z), rounded to the element type as the separate pass does it
+template <int BR, bool KC, int NT> struct StagedSlope {
+    typedef Staged<BR, KC, NT> S;
+    S g, z;
+    int act;
+    float slope;
+    __device__ __forceinline__ void init(const Operand &dy, const Operand &saved, int act_, float slope_, int64_t row0, int64_t nrows, int64_t k0)
+    {
+        act = act_;
+        slope = slope_;
+        g.init(dy, row0, nrows, k0);
+        if (act != AVC_ACT_NONE) z.init(saved, row0, nrows, k0);
+    }
+    __device__ __forceinline__ void load(int64_t kleft, int tid)
+    {
+        g.load(kleft, tid);
+        if (act != AVC_ACT_NONE) z.load(kleft, tid);
+    }
+    __device__ __forceinline__ void store(char *lds, int tid) const
+    {
 #pragma unroll
-                for (int k = 0; k < 3; ++k) *reinterpret_cast<bf16x8 *>(dst + k * L::BYTES) = s[k];
-            } else {
-                *reinterpret_cast<elem8 *>(dst) = v[i];
+        for (int i = 0; i < S::N; ++i) {
+            elem8 x = g.v[i];
+            if (act != AVC_ACT_NONE) {
+                float zs[8], sl[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) zs[j] = (float)z.v[i][j];
+                slope_run<8>(zs, sl, act, slope);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = (elem_t)((float)x[j] * sl[j]);
             }
+            S::put(lds, i * NT + tid, x);
         }
     }
 };
@@ -276,20 +316,21 @@ template <int VEC> __device__ __forceinline__ void store_run(elem_t *dst, const 
 // Steps of LDS.  float32's middle tile keeps one (48 KB), so that three workgroups share a CU and fill each other's waits; everything else two.
 constexpr int stages(int BM) { return IS_F32 && BM == 128 ? 1 : 2; }
 
-template <int BM, int BN, int WM, int WN, bool PKC, bool QKC, bool DMA>
-__global__ __launch_bounds__(WM * WN * 64, IS_F32 && BM == 128 ? 3 : 2) void tile_kernel(const TileArgs a)
+// DZ: P is dy, and what is multiplied is dy act'(saved)
+struct Slope { Operand saved; int act; float slope; };
+
+template <int BM, int BN, int WM, int WN, bool PKC, bool QKC, bool DMA, bool DZ>
+__device__ __forceinline__ void tile_body(const TileArgs &a, const Slope &dz, unsigned id, unsigned total, char *smem)
 {
     constexpr int NW = WM * WN, NT = NW * 64, FM = BM / WM / 16, FN = BN / WN / 16;
     typedef Tile<BM, PKC> LP;
     typedef Tile<BN, QKC> LQ;
     constexpr int STAGE = NP * (LP::BYTES + LQ::BYTES), STAGES = stages(BM);
-    extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
     // Workgroups go to the 8 XCDs in turn; give every XCD a contiguous run of tiles, walked in bands of 8 tile rows, so that its L2 sees the same rows and columns again.
-    unsigned id = blockIdx.x;
     {
-        const unsigned total = gridDim.x, per = total >> 3, rem = total & 7, x = id & 7;
+        const unsigned per = total >> 3, rem = total & 7, x = id & 7;
         id = x * per + min(x, rem) + (id >> 3);
     }
     const unsigned tiles = (unsigned)a.tiles_m * (unsigned)a.tiles_n, split = id / tiles, t = id % tiles;
@@ -352,9 +393,10 @@ __global__ __launch_bounds__(WM * WN * 64, IS_F32 && BM == 128 ? 3 : 2) void til
             }
         }
     } else {
-        Staged<BM, PKC, NT> sp;
+        typename std::conditional<DZ, StagedSlope<BM, PKC, NT>, Staged<BM, PKC, NT>>::type sp;
         Staged<BN, QKC, NT> sq;
-        sp.init(a.P, m0, a.M, k0);
+        if constexpr (DZ) sp.init(a.P, dz.saved, dz.act, dz.slope, m0, a.M, k0);
+        else sp.init(a.P, m0, a.M, k0);
         sq.init(a.Q, n0, a.N, k0);
         if (steps > 0) {
             sp.load(kend - k0, tid);
@@ -456,6 +498,50 @@ __global__ __launch_bounds__(WM * WN * 64, IS_F32 && BM == 128 ? 3 : 2) void til
     }
 }
 
+template <int BM, int BN, int WM, int WN, bool PKC, bool QKC, bool DMA>
+__global__ __launch_bounds__(WM * WN * 64, IS_F32 && BM == 128 ? 3 : 2) void tile_kernel(const TileArgs a)
+{
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    tile_body<BM, BN, WM, WN, PKC, QKC, DMA, false>(a, Slope{}, blockIdx.x, gridDim.x, smem);
+}
+
+// The whole backward pass of a small layer in one launch: workgroups for the tiles of dx, then for those of dw, then for 16 columns of db each.  The three read dy and z for
+// themselves and form dz on the way into LDS.
+template <bool XKC> __global__ __launch_bounds__(256, 2) void small_backward_kernel(const SmallArgs a)
+{
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const unsigned id = blockIdx.x, ndx = (unsigned)a.dx.tiles_m * (unsigned)a.dx.tiles_n, ndw = (unsigned)a.dw.tiles_m * (unsigned)a.dw.tiles_n;
+    if (id < ndx) {
+        tile_body<64, 64, 2, 2, true, false, false, true>(a.dx, Slope{Operand{a.saved, a.ld_saved, 1}, a.act, a.slope}, id, ndx, smem);
+    } else if (id < ndx + ndw) {
+        tile_body<64, 64, 2, 2, false, !XKC, false, true>(a.dw, Slope{Operand{a.saved, a.ld_saved, 0}, a.act, a.slope}, id - ndx, ndw, smem);
+    } else {
+        float(*red)[17] = reinterpret_cast<float(*)[17]>(smem);
+        const int lx = threadIdx.x & 15, ly = threadIdx.x >> 4;
+        const int64_t n = (int64_t)(id - ndx - ndw) * 16 + lx, nc = min(n, a.N - 1);
+        const elem_t *dy = (const elem_t *)a.dy + nc, *z = (const elem_t *)a.saved + nc;
+        float s = 0.f;
+        for (int64_t m = ly; m < a.M; m += 16 * 4) {
+            float g[4], zs[4], sl[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int64_t r = min(m + 16 * j, a.M - 1);
+                g[j] = (float)dy[r * a.lddy];
+                zs[j] = a.act != AVC_ACT_NONE ? (float)z[r * a.ld_saved] : 0.f;
+            }
+            slope_run<4>(zs, sl, a.act, a.slope);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s += m + 16 * j < a.M ? g[j] * sl[j] : 0.f;
+        }
+        red[ly][lx] = s;
+        __syncthreads();
+        if (ly || n >= a.N) return;
+#pragma unroll
+        for (int y = 1; y < 16; ++y) s += red[y][lx];
+        ((elem_t *)a.db)[n] = (elem_t)s;
+    }
+}
+
 template <int BM, int BN, int WM, int WN, bool PKC, bool QKC, bool DMA> int launch_one(const TileArgs &a, hipStream_t s)
 {
     constexpr int LDS = stages(BM) * NP * (Tile<BM, PKC>::BYTES + Tile<BN, QKC>::BYTES);
@@ -492,6 +578,15 @@ template <bool DMA> int launch_shape(const TileArgs &a, int tile, hipStream_t s)
     return launch_layout<64, 64, 2, 2, DMA>(a, s);
 }
 
+template <bool XKC> int launch_small(const SmallArgs &a, unsigned blocks, hipStream_t s)
+{
+    constexpr int A = Tile<64, true>::BYTES + Tile<64, false>::BYTES, B = Tile<64, false>::BYTES + Tile<64, !XKC>::BYTES, LDS = 2 * NP * (A > B ? A : B);
+    static_assert(LDS <= 64 * 1024, "within the default limit");
+    hipLaunchKernelGGL(small_backward_kernel<XKC>, dim3(blocks), dim3(256), LDS, s, a);
+    AVC_HIP(hipGetLastError());
+    return AVC_OK;
+}
+
 // the direct loads' conditions: whole 16-byte pieces, aligned, and a tile's offsets within 31 bits
 bool direct_ok(const Operand &o, int64_t rows, int64_t K)
 {
@@ -500,6 +595,11 @@ bool direct_ok(const Operand &o, int64_t rows, int64_t K)
 }
 
 }  // namespace
+
+int AVC_LAUNCH_SMALL(const SmallArgs &a, unsigned blocks, bool x_kc, hipStream_t s)
+{
+    return x_kc ? launch_small<true>(a, blocks, s) : launch_small<false>(a, blocks, s);
+}
 
 int AVC_LAUNCH(const TileArgs &a, int tile, hipStream_t s)
 {
