@@ -303,11 +303,12 @@ static int check_linear(const char *who, int64_t M, int64_t N, int64_t K, int dt
                 (long long)N, (long long)K);
     return AVC_OK;
 }
-static int check_x(const char *who, int64_t x_row, int64_t x_col, int64_t M, int64_t K)
+constexpr int64_t ROW_STRIDE_TOP = (int64_t)1 << 22;        // a tile's 256 rows are addressed with 32-bit offsets from its corner
+static int check_x(const char *who, int64_t x_row, int64_t x_col, int64_t col_top)
 {
-    constexpr int64_t TOP = (int64_t)1 << 40;
-    AVC_REQUIRE((x_col == 1 || x_row == 1) && x_row >= 0 && x_col >= 0 && x_row < TOP && x_col < TOP, AVC_ERR_ARG, "%s: one of x's strides has to be 1 and none negative (got %lld, %lld)", who,
-                (long long)x_row, (long long)x_col);
+    AVC_REQUIRE((x_col == 1 || x_row == 1) && x_row >= 0 && x_col >= 0, AVC_ERR_ARG, "%s: one of x's strides has to be 1 and none negative (got %lld, %lld)", who, (long long)x_row,
+                (long long)x_col);
+    AVC_REQUIRE(x_col == 1 ? x_row < ROW_STRIDE_TOP : x_col < col_top, AVC_ERR_ARG, "%s: x's stride of %lld elements is too large", who, (long long)(x_col == 1 ? x_row : x_col));
     return AVC_OK;
 }
 static avc::lin::Operand x_operand(const void *x, int64_t x_row, int64_t x_col) { return x_col == 1 ? avc::lin::Operand{x, x_row, 1} : avc::lin::Operand{x, x_col, 0}; }
@@ -332,7 +333,7 @@ int avc_linear_workspace(int64_t M, int64_t N, int64_t K, int dtype, int64_t x_r
 {
     AVC_REQUIRE(bytes, AVC_ERR_ARG, "avc_linear_workspace: NULL argument");
     if (int rc = check_linear("avc_linear_workspace", M, N, K, dtype)) return rc;
-    if (int rc = check_x("avc_linear_workspace", x_row, x_col, M, K)) return rc;
+    if (int rc = check_x("avc_linear_workspace", x_row, x_col, (int64_t)1 << 25)) return rc;
     *bytes = (int64_t)lin::forward_workspace(M, N, K, dtype, x_col == 1);
     return AVC_OK;
 }
@@ -342,9 +343,10 @@ int avc_linear(avc_ctx *ctx, const void *x, int64_t x_row, int64_t x_col, const 
 {
     if (int rc = check_linear("avc_linear", M, N, K, dtype)) return rc;
     AVC_REQUIRE(ctx && (!M || (x && w && y)), AVC_ERR_ARG, "avc_linear: NULL argument");
-    if (int rc = check_x("avc_linear", x_row, x_col, M, K)) return rc;
+    if (int rc = check_x("avc_linear", x_row, x_col, (int64_t)1 << 25)) return rc;
     AVC_REQUIRE(act >= AVC_ACT_NONE && act <= AVC_ACT_SILU, AVC_ERR_ARG, "avc_linear: unknown activation %d", act);
-    AVC_REQUIRE(ldw >= 0 && ldy >= N && (!res || ldr >= 0) && (!z || ldz >= N), AVC_ERR_ARG, "avc_linear: a row stride is negative, or an output's shorter than its row");
+    AVC_REQUIRE(ldw >= 0 && ldw < ROW_STRIDE_TOP && ldy >= N && (!res || ldr >= 0) && (!z || ldz >= N), AVC_ERR_ARG,
+                "avc_linear: a row stride is negative or too large, or an output's shorter than its row");
     AVC_REQUIRE(((uintptr_t)workspace & 15) == 0 && workspace_bytes >= (int64_t)lin::forward_workspace(M, N, K, dtype, x_col == 1) && (workspace || !workspace_bytes), AVC_ERR_CAPACITY,
                 "avc_linear: needs %lld bytes of 16-byte aligned workspace, got %lld", (long long)lin::forward_workspace(M, N, K, dtype, x_col == 1), (long long)workspace_bytes);
     if (!M) return AVC_OK;
@@ -368,8 +370,9 @@ int avc_linear_backward(avc_ctx *ctx, const void *dy, int64_t lddy, const void *
     AVC_REQUIRE(act >= AVC_ACT_NONE && act <= AVC_ACT_SILU, AVC_ERR_ARG, "avc_linear_backward: unknown activation %d", act);
     AVC_REQUIRE(ctx && (!M || (dy && (!dw || x) && (!dx || w) && (act == AVC_ACT_NONE || saved))), AVC_ERR_ARG, "avc_linear_backward: NULL argument");
     if (dw)
-        if (int rc = check_x("avc_linear_backward", x_row, x_col, M, K)) return rc;
-    AVC_REQUIRE(lddy >= 0 && ldw >= 0 && (act == AVC_ACT_NONE || ld_saved >= 0), AVC_ERR_ARG, "avc_linear_backward: a row stride is negative");
+        if (int rc = check_x("avc_linear_backward", x_row, x_col, ROW_STRIDE_TOP)) return rc;
+    AVC_REQUIRE(lddy >= 0 && lddy < ROW_STRIDE_TOP && N < ROW_STRIDE_TOP && (!dx || (ldw >= 0 && ldw < ROW_STRIDE_TOP)) && (act == AVC_ACT_NONE || (ld_saved >= 0 && ld_saved < ROW_STRIDE_TOP)),
+                AVC_ERR_ARG, "avc_linear_backward: a row stride is negative or too large");
     AVC_REQUIRE(((uintptr_t)workspace & 15) == 0 && workspace_bytes >= (int64_t)lin::backward_workspace(M, N, K, dtype) && (workspace || !workspace_bytes), AVC_ERR_CAPACITY,
                 "avc_linear_backward: needs %lld bytes of 16-byte aligned workspace, got %lld", (long long)lin::backward_workspace(M, N, K, dtype), (long long)workspace_bytes);
     AVC_ON_DEVICE(ctx);
@@ -380,7 +383,7 @@ static int check_norm(const char *who, int64_t M, int64_t C, int dtype)
 {
     constexpr int64_t TOP = (int64_t)1 << 31;
     AVC_REQUIRE(dtype >= AVC_F32 && dtype <= AVC_F16, AVC_ERR_ARG, "%s: unknown dtype %d", who, dtype);
-    AVC_REQUIRE(M >= 0 && C >= 1 && M < TOP && C < TOP, AVC_ERR_ARG, "%s: need 0 <= M, 1 <= C, both below 2^31 (got %lld, %lld)", who, (long long)M, (long long)C);
+    AVC_REQUIRE(M >= 0 && C >= 1 && M < TOP && C < (int64_t)1 << 26, AVC_ERR_ARG, "%s: need 0 <= M < 2^31, 1 <= C < 2^26 (got %lld, %lld)", who, (long long)M, (long long)C);
     return AVC_OK;
 }
 

@@ -71,7 +71,7 @@ __global__ __launch_bounds__(TPR ? TPR : 256) void norm_kernel(const T *__restri
 {
     __shared__ float red[16];
     const int tpr = TPR ? TPR : 1 << tpr_log, lane = threadIdx.x & (tpr - 1), rows = TPR ? 1 : 256 >> tpr_log, sub = TPR ? 0 : threadIdx.x >> tpr_log;
-    const float inv = 1.f / (float)C;
+    const float count = (float)C;                                        // divided by, not multiplied with 1 / C: a row of equal values has that value as its mean
     for (int64_t m0 = (int64_t)blockIdx.x * rows * R; m0 < M; m0 += (int64_t)gridDim.x * rows * R) {
         float v[R][NCH][V], mean[R], rstd[R];
 #pragma unroll
@@ -89,7 +89,7 @@ __global__ __launch_bounds__(TPR ? TPR : 256) void norm_kernel(const T *__restri
 #pragma unroll
                 for (int j = 0; j < V; ++j) s += j >= first ? v[r][c][j] : 0.f;
             }
-            mean[r] = row_sum<TPR>(s, tpr, red) * inv;
+            mean[r] = row_sum<TPR>(s, tpr, red) / count;
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -103,7 +103,7 @@ __global__ __launch_bounds__(TPR ? TPR : 256) void norm_kernel(const T *__restri
                     s += j >= first ? v[r][c][j] * v[r][c][j] : 0.f;
                 }
             }
-            rstd[r] = 1.f / sqrtf(row_sum<TPR>(s, tpr, red) * inv + eps);
+            rstd[r] = 1.f / sqrtf(row_sum<TPR>(s, tpr, red) / count + eps);
         }
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {

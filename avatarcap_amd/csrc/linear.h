@@ -102,7 +102,10 @@ __device__ __forceinline__ float log1p_unit(float t)
 __device__ __forceinline__ float normal_tail(float z, float &e)
 {
     const float t = rcp(fmaf(fabsf(z), 0.35355339059327379f, 1.f));
-    e = exp_acc(-0.5f * z * z);
+    // the exponent in two parts, as exp_acc takes it, with what the square's rounding misses: rounded to one part it would cost z^2 / 2 steps
+    constexpr float L = -0.721347510814666748046875f, LT = -9.62981516750005e-9f;
+    const float q = z * z, h = q * L, l = fmaf(q, L, -h) + fmaf(q, LT, fmaf(z, z, -q) * L), x = __builtin_amdgcn_exp2f(h);
+    e = q < 200.f ? fmaf(x, l * 0.69314718055994531f, x) : 0.f;             // below float32's range from 175 on
     float p = -0.0295328330f;
     p = fmaf(p, t, 0.1422793418f); p = fmaf(p, t, -0.2435828894f); p = fmaf(p, t, 0.1390137970f); p = fmaf(p, t, -0.0132990004f);
     p = fmaf(p, t, 0.1013374850f); p = fmaf(p, t, 0.1215534136f); p = fmaf(p, t, 0.1411874443f); p = fmaf(p, t, 0.1410432160f);

@@ -307,10 +307,11 @@ inline int esize(int dtype) { return dtype == AVC_F32 ? 4 : 2; }
 // The time of a launch is estimated for every tile shape and a ladder of splits, and the least taken.  With W workgroups on the fullest CU, `occ` of them at a time, and S steps of
 // k each:   launch + max(ceil(W / occ) (S lone_step + lone), W (S step + rest)) + the splits' sums written, read and reduced.
 // `lone_*` is a workgroup's own latency, `step` / `rest` its share of a busy CU (matrix rate; writing the tile out).  Constants in us, fitted to 1020 timed launches of 17 shapes
-// (64 .. 262144 rows, 64 .. 4096 columns and k, all three products): the choice came out 2 % slower than the best of all tiles and splits in the mean, 38 % at worst (a 14 us call).
+// (64 .. 262144 rows, 64 .. 4096 columns and k, all three products): the choice came out 2 % slower than the best of all tiles and splits in the mean, 63 % at worst (64 -> 1024
+// float32 on 33000 rows, 77 us for 48).
 struct TileCost { int occ; double lone_step, lone, step, rest; };
-constexpr TileCost COST_16[3] = {{1, 1.62, 7.0, 0.01, 11.1}, {2, 0.91, 1.9, 0.47, 3.3}, {5, 0.64, 0.0, 0.20, 1.0}};
-constexpr TileCost COST_F32[3] = {{1, 2.67, 5.4, 0.00, 12.0}, {3, 3.64, 1.7, 1.57, 4.3}, {3, 0.89, 1.7, 0.57, 1.0}};
+constexpr TileCost COST_16[3] = {{1, 1.61, 6.9, 0.20, 11.2}, {2, 0.88, 2.1, 0.46, 3.2}, {5, 0.61, 0.0, 0.20, 1.0}};
+constexpr TileCost COST_F32[3] = {{1, 1.99, 6.9, 2.75, 3.6}, {3, 2.80, 3.1, 1.62, 3.1}, {3, 0.92, 1.8, 0.58, 1.0}};
 constexpr int SPLITS[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256};
 
 struct Plan { int tile, tiles_m, tiles_n, splits; int64_t kper; double us; };
@@ -466,18 +467,20 @@ size_t forward_workspace(int64_t M, int64_t N, int64_t K, int dtype, bool x_kc)
     return M && route(M, N, x_kc) == ROUTE_TILE ? product_bytes(M, N, K, dtype) : 0;
 }
 
-// Layers whose gradients are a few dozen tiles with short sums: the launches would cost more than the work, so one launch does it all (no workspace).  17 x 33 -> 65 with a bias:
-// one launch instead of three.
-static bool small_backward(int64_t M, int64_t N, int64_t K)
+// Layers whose gradients are no more tiles than the chip has CUs, with sums of at most eight steps: the launches cost more than the work (20.6 us of host time and three launches
+// against 13.2 us and one for 16 x 24 -> 7), so one launch does it all, without workspace.  Longer sums are faster split over several workgroups (float32 gradients of 128 x 1024
+// -> 1024 rows: 33 us here, 11 us split).
+static bool small_backward(int64_t M, int64_t N, int64_t K, int dtype)
 {
-    return M >= 1 && M <= 512 && N <= 1024 && cdiv(N, 64) * cdiv(K, 64) <= 256 && cdiv(M, 64) * cdiv(K, 64) <= 256;
+    const int64_t longest = 8 * tile_bk(dtype);
+    return M >= 1 && M <= longest && N <= longest && cdiv(N, 64) * cdiv(K, 64) <= 256 && cdiv(M, 64) * cdiv(K, 64) <= 256;
 }
 
 struct BackwardSpace { size_t dz, strips, partial, total; };
 static BackwardSpace backward_space(int64_t M, int64_t N, int64_t K, int dtype)
 {
     BackwardSpace w{};
-    if (small_backward(M, N, K)) return w;
+    if (small_backward(M, N, K, dtype)) return w;
     w.dz = align256((size_t)M * N * esize(dtype));
     w.strips = align256(sizeof(float) * (size_t)strips_for(M, N, dtype) * N);
     w.partial = product_bytes(N, K, M, dtype);
@@ -501,7 +504,7 @@ int backward(const void *dy, int64_t lddy, const Operand &x, const void *w, int6
              void *dx, void *dw, void *db, void *ws, hipStream_t s)
 {
     const Epilogue none{nullptr, nullptr, 0, nullptr, 0, AVC_ACT_NONE, 0.f};
-    if (small_backward(M, N, K)) {
+    if (small_backward(M, N, K, dtype)) {
         SmallArgs a{};
         auto tiles = [](TileArgs &t, const Operand &P, const Operand &Q, int64_t m, int64_t n, int64_t k, void *out) {
             t = TileArgs{P, Q, m, n, k, out, n, Epilogue{nullptr, nullptr, 0, nullptr, 0, AVC_ACT_NONE, 0.f}, nullptr, k, (int)cdiv(m, 64), (int)cdiv(n, 64), 1};

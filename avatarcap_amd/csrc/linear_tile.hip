@@ -68,25 +68,30 @@ template <int BR, bool KC> struct Tile {
     // byte of piece p of row `row`
     __device__ static __forceinline__ int at(int row, int p) { return row * ROW_BYTES + ((p ^ swizzle(row)) << 4); }
 
-    // fragment t of the wave whose rows start at r0: the lane's 8 values of k step ks
-    __device__ static __forceinline__ half8 fragment(const char *base, int r0, int t, int ks, int lane)
+    // A wave's reads: fragment t holds the rows r0 + 16 t .., the lane's 8 values of k step ks.  Offsets are two numbers per lane and an XOR with constants; `x` is to be passed
+    // through fresh() once per step, or the compiler keeps every fragment's address in a register of its own through the loop (and spills).
+    struct Reader { unsigned row, x; };
+    __device__ static __forceinline__ Reader reader(int r0, int lane)
     {
         const int l16 = lane & 15, q = lane >> 4;
+        if constexpr (KC) return Reader{(unsigned)((r0 + l16) * ROW_BYTES), (unsigned)((q ^ swizzle(l16)) << 4)};
+        // ds_read_b64_tr_b16: within 16 lanes, lane 4 a + c supplies the address of 4 adjacent values of k row a, and lane i receives the 4 k values of column i
+        const int a = l16 >> 2, c = l16 & 3, k = 8 * q + a;             // (the swizzle does not look at bit 2 of k)
+        return Reader{(unsigned)(k * ROW_BYTES + ((c & 1) << 3)), (unsigned)(((r0 >> 3) + (c >> 1)) ^ swizzle(k)) << 4};
+    }
+    __device__ static __forceinline__ Reader fresh(Reader r)
+    {
+        asm volatile("" : "+v"(r.x));
+        return r;
+    }
+    __device__ static __forceinline__ half8 fragment(const char *base, const Reader &r, int t, int ks)
+    {
         if constexpr (KC) {
-            const int row = r0 + 16 * t + l16;
-            return *reinterpret_cast<const half8 *>(base + at(row, ks * 4 + q));
+            return *reinterpret_cast<const half8 *>(base + ((r.x ^ (unsigned)(ks * 64)) + r.row) + t * 16 * ROW_BYTES);
         } else {
-            // ds_read_b64_tr_b16: within 16 lanes, lane 4 a + c supplies the address of 4 adjacent values of k row a, and lane i receives the 4 k values of column i
-            const int a = l16 >> 2, c = l16 & 3;
-            const int col = r0 + 16 * t + 4 * c;
-            s16x4 v[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int k = ks * 32 + 8 * q + 4 * h + a;
-                const char *p = base + at(k, col >> 3) + ((col & 4) << 1);
-                v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p);
-            }
-            s16x8 w = {v[0][0], v[0][1], v[0][2], v[0][3], v[1][0], v[1][1], v[1][2], v[1][3]};
+            const char *p = base + ((r.x ^ (unsigned)(t * 32)) + r.row) + ks * 32 * ROW_BYTES;
+            const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p), v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + 4 * ROW_BYTES));
+            const s16x8 w = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
             return __builtin_bit_cast(half8, w);
         }
     }
@@ -154,47 +159,88 @@ template <typename X> __device__ __forceinline__ void split3(const X &x, bf16x8 
     }
 }
 
+// x[j] <- x[j + s], zeros from the top; s = 0 .. 8
+__device__ __forceinline__ void shift_down(f32x8 &x, int s)
+{
+#pragma unroll
+    for (int b = 8; b >= 1; b >>= 1)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = s & b ? (j + b < 8 ? x[j + b < 8 ? j + b : j] : 0.f) : x[j];
+}
+template <typename X> __device__ __forceinline__ void shift_down(X &v, int s)             // 16-bit elements, two to a word
+{
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    u32x4 x = __builtin_bit_cast(u32x4, v);
+#pragma unroll
+    for (int b = 4; b >= 1; b >>= 1)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = s & (2 * b) ? (j + b < 4 ? x[j + b < 4 ? j + b : j] : 0u) : x[j];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = s & 1 ? (j < 3 ? __builtin_amdgcn_alignbit(x[j < 3 ? j + 1 : 3], x[j], 16) : x[j] >> 16) : x[j];
+    v = __builtin_bit_cast(X, x);
+}
+
 template <int BR, bool KC, int NT> struct Staged {
     typedef Tile<BR, KC> L;
     static constexpr int N = (L::BYTES / 16 + NT - 1) / NT;             // pieces of 8 values per thread
     static constexpr bool FULL = L::BYTES / 16 % NT == 0;
     elem8 v[N];
-    const elem_t *base;                                                 // element (row0, k0)
-    int64_t ld, rows;                                                   // rows left from row0 on
-    __device__ __forceinline__ void init(const Operand &o, int64_t row0, int64_t nrows, int64_t k0)
+    unsigned off[N];                                                    // bytes from `base` to the thread's pieces (the host keeps the strides small enough)
+    const char *base;                                                   // element (row0, k0), the same for all threads
+    int64_t ld, rows, axis;                                             // bytes; rows left from row0 on; length of the contiguous axis
+    __device__ __forceinline__ void init(const Operand &o, int64_t row0, int64_t nrows, int64_t k0, int64_t K, int tid)
     {
-        ld = o.ld;
+        axis = KC ? K : nrows;
+        ld = o.ld * (int64_t)sizeof(elem_t);
         rows = nrows - row0;
-        base = (const elem_t *)o.p + (KC ? row0 * ld + k0 : k0 * ld + row0);
+        base = (const char *)o.p + (KC ? row0 * ld + k0 * (int64_t)sizeof(elem_t) : k0 * ld + row0 * (int64_t)sizeof(elem_t));
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int id = i * NT + tid, r = id / L::PIECES, p = id % L::PIECES;
+            // rows past the end repeat the last one: their outputs are not stored
+            const unsigned row = KC ? (unsigned)min((int64_t)r, rows - 1) : (unsigned)(FULL ? r : min(r, BK - 1));
+            off[i] = row * (unsigned)ld + p * 8 * (unsigned)sizeof(elem_t);
+        }
     }
-    // No branch depends on a lane: a branch around a load would make every load wait for the one before it.  Rows past the end repeat the last one (their outputs are not
-    // stored); a step that ends inside a piece takes its values one by one, from clamped indices, and zeroes those past the end.
+    // No branch depends on a lane: a branch around a load would make every load wait for the one before it.  Where a step or a tile ends inside the contiguous axis, the pieces
+    // that would pass its end are read further back, to end with it, and shifted down, zeros behind.  Only axes of fewer than 8 values in all are read one by one.
     __device__ __forceinline__ void load(int64_t kleft, int tid)
     {
         const bool whole = KC ? kleft >= BK : (kleft >= BK && rows >= BR);
         if (whole) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int id = i * NT + tid, r = id / L::PIECES, p = id % L::PIECES;
-                const int64_t row = KC ? min((int64_t)r, rows - 1) : (FULL ? r : min(r, BK - 1));
-                __builtin_memcpy(&v[i], base + row * ld + p * 8, sizeof v[i]);
-            }
+            for (int i = 0; i < N; ++i) __builtin_memcpy(&v[i], base + off[i], sizeof v[i]);
         } else {
-            const int64_t inner = KC ? kleft : rows, outer = KC ? rows : kleft;       // both >= 1
+            const int inner = (int)min(KC ? kleft : rows, (int64_t)BR + BK), outer = (int)min(KC ? rows : kleft, (int64_t)BR + BK);      // both >= 1
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const int id = i * NT + tid, r = id / L::PIECES, p = id % L::PIECES;
-                const elem_t *src = base + min((int64_t)r, outer - 1) * ld;
-                elem8 x;
+                const int id = i * NT + tid, r = id / L::PIECES, p = id % L::PIECES * 8;
+                const char *row = base + (unsigned)min(r, outer - 1) * (unsigned)ld;
+                int s = 0;
+                if (axis >= 8) {
+                    const int start = min(p, inner - 8);
+                    s = r < outer ? min(p - start, 8) : 8;
+                    __builtin_memcpy(&v[i], row + start * (int)sizeof(elem_t), sizeof v[i]);
+                    shift_down(v[i], s);
+                    __builtin_amdgcn_sched_barrier(0);
+                } else {
+                    typedef typename std::conditional<IS_F32, unsigned, unsigned short>::type bits_t;
+                    unsigned raw[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = src[min((int64_t)(p * 8 + j), inner - 1)];
+                    for (int j = 0; j < 8; ++j) {
+                        raw[j] = *reinterpret_cast<const bits_t *>(row + min(p + j, inner - 1) * (int)sizeof(elem_t));
+                    }
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (p * 8 + j >= inner || r >= outer) x[j] = (elem_t)0.f;
-                v[i] = x;
+                    for (int j = 0; j < 8; ++j) {
+                        asm volatile("" : "+v"(raw[j]));                // the load stays outside of the choice, or it becomes a branch
+                        if (p + j >= inner || r >= outer) raw[j] = 0;
+                        v[i][j] = __builtin_bit_cast(elem_t, (bits_t)raw[j]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
         }
-        base += KC ? (int64_t)BK : BK * ld;
+        base += KC ? (int64_t)BK * (int64_t)sizeof(elem_t) : BK * ld;
     }
     __device__ static __forceinline__ void put(char *lds, int id, const elem8 &x)
     {
@@ -212,7 +258,10 @@ template <int BR, bool KC, int NT> struct Staged {
     __device__ __forceinline__ void store(char *lds, int tid) const
     {
 #pragma unroll
-        for (int i = 0; i < N; ++i) put(lds, i * NT + tid, v[i]);
+        for (int i = 0; i < N; ++i) {
+            put(lds, i * NT + tid, v[i]);
+            if (NP > 1) __builtin_amdgcn_sched_barrier(0);             // one piece's planes at a time
+        }
     }
 };
 
@@ -222,12 +271,12 @@ template <int BR, bool KC, int NT> struct StagedSlope {
     S g, z;
     int act;
     float slope;
-    __device__ __forceinline__ void init(const Operand &dy, const Operand &saved, int act_, float slope_, int64_t row0, int64_t nrows, int64_t k0)
+    __device__ __forceinline__ void init(const Operand &dy, const Operand &saved, int act_, float slope_, int64_t row0, int64_t nrows, int64_t k0, int64_t K, int tid)
     {
         act = act_;
         slope = slope_;
-        g.init(dy, row0, nrows, k0);
-        if (act != AVC_ACT_NONE) z.init(saved, row0, nrows, k0);
+        g.init(dy, row0, nrows, k0, K, tid);
+        if (act != AVC_ACT_NONE) z.init(saved, row0, nrows, k0, K, tid);
     }
     __device__ __forceinline__ void load(int64_t kleft, int tid)
     {
@@ -254,31 +303,36 @@ template <int BR, bool KC, int NT> struct StagedSlope {
 
 // ---- the tile's products ------------------------------------------------------------------------------------------------------------------------------------
 template <int FM, int FN, typename LP, typename LQ>
-__device__ __forceinline__ void compute(const char *P, const char *Q, int pr0, int qr0, int lane, f32x4 (&acc)[FM][FN])
+__device__ __forceinline__ void compute(const char *P, const char *Q, typename LP::Reader rp, typename LQ::Reader rq, f32x4 (&acc)[FM][FN])
 {
+    rp = LP::fresh(rp);
+    rq = LQ::fresh(rq);
 #pragma unroll
     for (int ks = 0; ks < BK / 32; ++ks) {
 #pragma unroll
         for (int a = 0; a < NP; ++a) {                                  // plane of Q: h with h m l, m with h m, l with h
             half8 q[FN];
 #pragma unroll
-            for (int t = 0; t < FN; ++t) q[t] = LQ::fragment(Q + a * LQ::BYTES, qr0, t, ks, lane);
+            for (int t = 0; t < FN; ++t) q[t] = LQ::fragment(Q + a * LQ::BYTES, rq, t, ks);
 #pragma unroll
-            for (int b = 0; b < NP - a; ++b)
+            for (int b = 0; b < NP - a; ++b) {
 #pragma unroll
                 for (int i = 0; i < FM; ++i) {
-                    const half8 p = LP::fragment(P + b * LP::BYTES, pr0, i, ks, lane);
+                    const half8 p = LP::fragment(P + b * LP::BYTES, rp, i, ks);
 #pragma unroll
                     for (int t = 0; t < FN; ++t) acc[i][t] = mfma(q[t], p, acc[i][t]);
                 }
+                if (NP > 1) __builtin_amdgcn_sched_barrier(0);         // or the reads of all nine plane pairs are hoisted and their registers spill
+            }
         }
     }
 }
 
-template <int F, typename L> __device__ __forceinline__ void read_fragments(half8 (&f)[F], const char *base, int r0, int ks, int lane)
+template <int F, typename L> __device__ __forceinline__ void read_fragments(half8 (&f)[F], const char *base, typename L::Reader r, int ks)
 {
+    r = L::fresh(r);
 #pragma unroll
-    for (int t = 0; t < F; ++t) f[t] = L::fragment(base, r0, t, ks, lane);
+    for (int t = 0; t < F; ++t) f[t] = L::fragment(base, r, t, ks);
 }
 template <int FM, int FN> __device__ __forceinline__ void multiply(const half8 (&p)[FM], const half8 (&q)[FN], f32x4 (&acc)[FM][FN])
 {
@@ -340,6 +394,9 @@ __device__ __forceinline__ void tile_body(const TileArgs &a, const Slope &dz, un
     const int steps = (int)((kend - k0 + BK - 1) / BK);
     const int pr0 = (wave / WN) * (BM / WM), qr0 = (wave % WN) * (BN / WN);
 
+    const typename LP::Reader rp = LP::reader(pr0, lane);
+    const typename LQ::Reader rq = LQ::reader(qr0, lane);
+
     f32x4 acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
@@ -367,12 +424,12 @@ __device__ __forceinline__ void tile_body(const TileArgs &a, const Slope &dz, un
                 dq.issue(smem + STAGE + LP::BYTES, kend - k0 - BK, wave, lane);
             }
             half8 p0[FM], q0[FN], p1[FM], q1[FN];
-            read_fragments<FN, LQ>(q0, smem + LP::BYTES, qr0, 0, lane);
-            read_fragments<FM, LP>(p0, smem, pr0, 0, lane);
+            read_fragments<FN, LQ>(q0, smem + LP::BYTES, rq, 0);
+            read_fragments<FM, LP>(p0, smem, rp, 0);
             for (int s = 0; s < steps; ++s) {
                 char *cur = smem + (s & 1) * STAGE, *nxt = smem + ((s + 1) & 1) * STAGE;
-                read_fragments<FN, LQ>(q1, cur + LP::BYTES, qr0, 1, lane);
-                read_fragments<FM, LP>(p1, cur, pr0, 1, lane);
+                read_fragments<FN, LQ>(q1, cur + LP::BYTES, rq, 1);
+                read_fragments<FM, LP>(p1, cur, rp, 1);
                 multiply(p0, q0, acc);
                 interleave<READS, FM * FN>();
                 __builtin_amdgcn_sched_barrier(0);
@@ -385,8 +442,8 @@ __device__ __forceinline__ void tile_body(const TileArgs &a, const Slope &dz, un
                     dq.issue(cur + LP::BYTES, kleft, wave, lane);
                 }
                 // (the last step reads what the other buffer holds and uses none of it)
-                read_fragments<FN, LQ>(q0, nxt + LP::BYTES, qr0, 0, lane);
-                read_fragments<FM, LP>(p0, nxt, pr0, 0, lane);
+                read_fragments<FN, LQ>(q0, nxt + LP::BYTES, rq, 0);
+                read_fragments<FM, LP>(p0, nxt, rp, 0);
                 multiply(p1, q1, acc);
                 interleave<READS, FM * FN>();
                 __builtin_amdgcn_sched_barrier(0);
@@ -395,9 +452,9 @@ __device__ __forceinline__ void tile_body(const TileArgs &a, const Slope &dz, un
     } else {
         typename std::conditional<DZ, StagedSlope<BM, PKC, NT>, Staged<BM, PKC, NT>>::type sp;
         Staged<BN, QKC, NT> sq;
-        if constexpr (DZ) sp.init(a.P, dz.saved, dz.act, dz.slope, m0, a.M, k0);
-        else sp.init(a.P, m0, a.M, k0);
-        sq.init(a.Q, n0, a.N, k0);
+        if constexpr (DZ) sp.init(a.P, dz.saved, dz.act, dz.slope, m0, a.M, k0, a.K, tid);
+        else sp.init(a.P, m0, a.M, k0, a.K, tid);
+        sq.init(a.Q, n0, a.N, k0, a.K, tid);
         if (steps > 0) {
             sp.load(kend - k0, tid);
             sq.load(kend - k0, tid);
@@ -413,7 +470,7 @@ __device__ __forceinline__ void tile_body(const TileArgs &a, const Slope &dz, un
                 sp.load(kleft, tid);
                 sq.load(kleft, tid);
             }
-            compute<FM, FN, LP, LQ>(cur, cur + NP * LP::BYTES, pr0, qr0, lane, acc);
+            compute<FM, FN, LP, LQ>(cur, cur + NP * LP::BYTES, rp, rq, acc);
         }
     }
 

@@ -40,10 +40,13 @@ def _check(who, first, **others):
             raise RuntimeError(f'{who}: {name} lives on {t.device}, x on {first.device}')
 
 
+_ROW_TOP, _COLUMN_TOP = 1 << 22, 1 << 25                                          # include/avcap.h: the strides that the kernels address
+
+
 def _rows(t):
-    """`t` (rows, columns) with adjacent columns, copied if they are not; rows may lie any distance apart."""
-    if t.stride(1) == 1 or t.shape[1] == 1:
-        return t if t.stride(0) >= 0 else t.contiguous()
+    """`t` (rows, columns) with adjacent columns, copied if they are not or the rows lie further apart than the kernels reach."""
+    if (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) < _ROW_TOP or t.shape[0] <= 1):
+        return t
     return t.contiguous()
 
 
@@ -51,12 +54,12 @@ def _row_stride(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _matrix(x):
+def _matrix(x, column_top=_COLUMN_TOP):
     """`x` (rows, columns) and its strides, one of which is 1: rows of adjacent values, or channel-first (a transposed view).  Copied otherwise."""
     m, k = x.shape
-    if k == 1 or x.stride(1) == 1:
+    if (k == 1 or x.stride(1) == 1) and (m <= 1 or x.stride(0) < _ROW_TOP):
         return x, _row_stride(x), 1
-    if x.stride(0) == 1 and m > 1:
+    if x.stride(0) == 1 and m > 1 and x.stride(1) < column_top:
         return x, 1, x.stride(1)
     x = x.contiguous()
     return x, k, 1
@@ -130,7 +133,7 @@ class _Linear(torch.autograd.Function):
         if need_x or need_w or need_b:
             (m, k), n, dt = x.shape, w.shape[0], DTYPES[dy.dtype]
             g = _rows(dy)
-            x, xr, xc = _matrix(x)
+            x, xr, xc = _matrix(x, _ROW_TOP)
             w = _rows(w)
             dx = g.new_empty((m, k)) if need_x else None
             dw = g.new_empty((n, k)) if need_w else None

@@ -164,7 +164,8 @@ enum avc_act { AVC_ACT_NONE = 0, AVC_ACT_RELU = 1, AVC_ACT_LEAKY_RELU = 2 /* z >
  *   x (M, K) at x[m * x_row + k * x_col], one of the two strides being 1 (x_col = 1: rows of points; x_row = 1: channel-first points as Conv1d has them)
  *   w (N, K) rows of K adjacent values, ldw apart;  bias (N) or NULL;  res (M, N), ldr apart, or NULL
  *   y (M, N), ldy apart;  z (M, N), ldz apart, or NULL: the value before the activation, which the backward pass reads.  y, z overlap no input (y may be res itself).
- * M >= 0, N, K >= 1.  A NaN or infinity of x or w reaches exactly the outputs it has a part in. */
+ * M >= 0, N, K >= 1.  A NaN or infinity of x or w reaches exactly the outputs it has a part in.
+ * Row strides (of x with x_col = 1, w, dy, saved) below 2^22 elements; x_col of channel-first points below 2^25 here, below 2^22 in the backward pass (AVC_ERR_ARG beyond). */
 int avc_linear_workspace(int64_t M, int64_t N, int64_t K, int dtype, int64_t x_row, int64_t x_col, int64_t *bytes);
 int avc_linear(avc_ctx *ctx, const void *x, int64_t x_row, int64_t x_col, const void *w, int64_t ldw, const void *bias, const void *res, int64_t ldr, int act, float slope, int64_t M,
                int64_t N, int64_t K, int dtype, void *y, int64_t ldy, void *z, int64_t ldz, void *workspace, int64_t workspace_bytes, avc_stream stream);
@@ -177,7 +178,7 @@ int avc_linear_backward(avc_ctx *ctx, const void *dy, int64_t lddy, const void *
                         float slope, int64_t M, int64_t N, int64_t K, int dtype, void *dx, void *dw, void *db, void *workspace, int64_t workspace_bytes, avc_stream stream);
 
 /* y = (x - mean) / sqrt(var + eps) * gamma + beta per row of C values (biased variance);  x, y (M, C) rows ldx / ldy apart (y may be x), gamma, beta (C) or NULL;
- * mean, rstd (M) float32, both or neither: the statistics, which the backward pass reads.  M >= 0, C >= 1, eps >= 0. */
+ * mean, rstd (M) float32, both or neither: the statistics, which the backward pass reads.  M >= 0, 1 <= C < 2^26, eps >= 0. */
 int avc_layer_norm(avc_ctx *ctx, const void *x, int64_t ldx, const void *gamma, const void *beta, float eps, int64_t M, int64_t C, int dtype, void *y, int64_t ldy, float *mean, float *rstd,
                    avc_stream stream);
 /* dx (M, C), lddx apart, dgamma (C), dbeta (C), any of them NULL; the workspace is needed for dgamma / dbeta only. */

@@ -39,7 +39,7 @@ def act64(z, act, slope):
         s = torch.sigmoid(z)
         return s, s * torch.sigmoid(-z)
     if act == 'tanh':
-        return torch.tanh(z), 1 - torch.tanh(z) ** 2
+        return torch.tanh(z), torch.cosh(z) ** -2
     if act == 'gelu':
         cdf = 0.5 * torch.erfc(-z / math.sqrt(2))
         return z * cdf, cdf + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
@@ -210,3 +210,377 @@ def test_norm_layouts_and_values(dtype):
     check_norm(300, 16500, dtype, pad=3, grad=False)
     check_norm(1200, 260, dtype, scale=0.01, shift=4.0 if dtype == torch.float32 else 0.02)
     check_norm(7, 512, dtype, scale=100.0, shift=-50.0, eps=1.0)
+
+
+# ---- values that a kernel must not lose ------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('m,k,n', [(3, 40, 33), (70, 40, 33), (70, 100, 140), (300, 264, 300)])
+def test_a_nan_or_infinity_reaches_its_own_row_only(m, k, n, dtype):
+    xd, x, w, b, r, dy = make(m, k, n, dtype)
+    for bad in (float('nan'), float('inf'), -float('inf')):
+        x2 = x.clone()
+        x2[m // 2, k - 1] = bad
+        y = linear(x2.cuda(), dev(w), dev(b)).cpu()
+        clean = linear(xd, dev(w), dev(b)).cpu()
+        keep = torch.arange(m) != m // 2
+        assert torch.equal(y[keep], clean[keep])
+        assert not bool(torch.isfinite(y[m // 2]).any())
+        if bad == bad:                                                       # w is nowhere zero: every output of the row is infinite, with the sign of the product
+            want = torch.sign(w[:, k - 1].double()) * bad
+            assert torch.equal(y[m // 2].double(), want)
+        w2 = w.clone()
+        w2[n - 1, 0] = bad
+        y = linear(xd, dev(w2), dev(b)).cpu()
+        assert torch.equal(y[:, :n - 1], clean[:, :n - 1]) and not bool(torch.isfinite(y[:, n - 1]).any())
+
+
+def test_float32_keeps_its_range():
+    """float32 goes through three bf16: the largest values, the smallest normal ones and sums that cancel.  In the last, w = 1 has a head alone, so the three non-zero x meet it as
+    9 exact products; the order of a sum is not fixed, and each of at most 9 additions is off by half a step of a partial sum below 2.01 |a|: 9 2^-24 2.01 |a|."""
+    g = torch.Generator().manual_seed(5)
+    for m, k, n in ((70, 64, 70), (300, 64, 300)):
+        x = torch.zeros(m, k)
+        x[:, 0] = 3.4e38 * torch.sign(torch.randn(m, generator=g))
+        x[:, 1] = 1.2e-38 * torch.rand(m, generator=g) * 3 + 1.2e-38
+        w = torch.zeros(n, k)
+        w[:, 0] = 0.5
+        y = linear(x.cuda(), w.cuda()).cpu()
+        assert torch.equal(y, (x[:, :1] * 0.5).expand(m, n))
+        w[:, 0], w[:, 1] = 0.0, 1.0
+        y = linear(x.cuda(), w.cuda()).cpu().double()
+        assert bool(((y - x[:, 1:2].double()).abs() <= 2.0 ** -126).all())   # the planes' tails are below the smallest normal and may be flushed
+        a = torch.randn(m, generator=g)
+        x = torch.zeros(m, k)
+        x[:, 0], x[:, 1], x[:, 2] = a, -a, 2.0 ** -20 * a
+        y = linear(x.cuda(), torch.ones(n, k).cuda()).cpu()
+        assert bool(((y.double() - x[:, 2:3].double()).abs() <= 9 * E32 * 2.01 * a.abs().double()[:, None]).all())
+
+
+@pytest.mark.parametrize('act', [a for a in ACTS])
+def test_activations_at_extreme_values(act):
+    """z itself is exact here (one product by 1): the activation and its slope over the range, against float64; both are bounded to 16 steps of float32 of max(|value|, 1e-30) plus
+    what half a step of z is worth, |z| <= 20 -> relative 2^-24 |z| of e^z.  An e^z below float32's smallest normal value 2^-126 may be zero, and silu and gelu multiply it by
+    |z|: `least`."""
+    z = torch.cat([torch.linspace(-30, 30, 4001), torch.tensor([0.0, -0.0, 1e-20, -1e-20, 1e-6, -1e-6, 20.0, 20.0001, 88.0, -88.0, 100.0, -100.0, 1e4, -1e4])])[:, None]
+    one = torch.ones(1, 1)
+    x, w = z.cuda().requires_grad_(), one.cuda()
+    y = linear(x, w, act=act)
+    y.backward(torch.ones_like(y))
+    v, s = act64(z.double(), act, 0.02)
+    rel = (16 + 3 * z.abs().double()) * E32
+    least = 1e-37 + 2.0 ** -126 * z.abs().double()
+    close(y, v, rel * v.abs() + least, act)
+    if act == 'gelu':                                                        # Phi + z phi cancels near its zero: the terms' size counts
+        cdf = 0.5 * torch.erfc(-z.double() / math.sqrt(2))
+        size = cdf + (z.double().abs() * torch.exp(-z.double() ** 2 / 2) / math.sqrt(2 * math.pi))
+    elif act == 'silu':
+        size = torch.sigmoid(z.double()) * (1 + z.double().abs() * torch.sigmoid(-z.double()))
+    else:
+        size = s.abs()
+    # float32's smallest normal: a slope below it may be zero.  gelu's e^(-z^2 / 2) carries z^2 / 2 steps
+    size = size * (1 + (z.double() ** 2 / 8 if act == 'gelu' else 0))
+    if act in ('relu', 'leaky_relu'):
+        keep = z != 0
+        assert torch.equal(x.grad.cpu()[keep], s.float()[keep])
+    else:
+        close(x.grad, s, rel * size + least, f"{act}'")
+    inf = torch.tensor([[float('inf')], [float('nan')]]).cuda()
+    got = linear(inf, w, act=act).cpu()
+    assert float(got[0, 0]) == (1.0 if act in ('sigmoid', 'tanh') else float('inf')) and bool(torch.isnan(got[1, 0]))
+
+
+def test_a_row_of_equal_values_has_a_finite_norm():
+    for dtype in DTYPES:
+        x = torch.full((5, 96), 3.0, dtype=dtype, device='cuda', requires_grad=True)
+        y = layer_norm(x)
+        assert bool((y == 0).all())
+        y.backward(torch.randn(5, 96, device='cuda').to(dtype))
+        assert bool(torch.isfinite(x.grad).all())
+        bad = torch.randn(4, 96, device='cuda').to(dtype)
+        good = layer_norm(bad.clone())
+        bad[1, 7], bad[2, 95] = float('nan'), float('inf')
+        y = layer_norm(bad)
+        assert bool(torch.isnan(y[1:3]).all()) and torch.equal(y[0], good[0]) and torch.equal(y[3], good[3])
+
+
+# ---- gradients against differences --------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('act', ['soft_plus', 'tanh', 'gelu', 'silu', 'sigmoid'])
+def test_gradients_are_the_slope_of_the_forward_pass(act):
+    """(f(v + h d) - f(v - h d)) / 2h along random directions, f the sum of y times fixed numbers in float64: truncation ~ h^2, rounding ~ 2^-24 |f terms| / h."""
+    g = torch.Generator().manual_seed(3)
+    x, w, b, r = (torch.randn(*s, generator=g).cuda().requires_grad_() for s in ((33, 20), (17, 20), (17,), (33, 17)))
+    c = torch.randn(33, 17, generator=g).cuda()
+    f = lambda *a: float((linear(a[0], a[1], a[2], act=act, residual=a[3]).double() * c.double()).sum())   # noqa: E731
+    grads = torch.autograd.grad(linear(x, w, b, act=act, residual=r), (x, w, b, r), c)
+    h = 2.0 ** -8
+    with torch.no_grad():
+        for i in range(4):
+            d = torch.randn(grads[i].shape, generator=g).cuda()
+            p, m = [x, w, b, r], [x, w, b, r]
+            p[i], m[i] = p[i] + h * d, m[i] - h * d
+            slope = (f(*p) - f(*m)) / (2 * h)
+            want = float((grads[i].double() * d.double()).sum())
+            scale = float((grads[i].double().abs() * d.double().abs()).sum())
+            assert abs(slope - want) < 3e-3 * scale, (act, i, slope, want)
+    x, gm, bt = (torch.randn(*s, generator=g).cuda().requires_grad_() for s in ((9, 40), (40,), (40,)))
+    c = torch.randn(9, 40, generator=g).cuda()
+    grads = torch.autograd.grad(layer_norm(x, gm, bt), (x, gm, bt), c)
+    with torch.no_grad():
+        for i in range(3):
+            d = torch.randn(grads[i].shape, generator=g).cuda()
+            p, m = [x, gm, bt], [x, gm, bt]
+            p[i], m[i] = p[i] + h * d, m[i] - h * d
+            slope = float(((layer_norm(*p).double() - layer_norm(*m).double()) * c.double()).sum()) / (2 * h)
+            want = float((grads[i].double() * d.double()).sum())
+            assert abs(slope - want) < 3e-3 * float((grads[i].double().abs() * d.double().abs()).sum()), (i, slope, want)
+
+
+# ---- how a program uses them ------------------------------------------------------------------------------------------------------------------------------------
+def test_shapes_views_and_partial_gradients():
+    g = torch.Generator().manual_seed(11)
+    x = torch.randn(2, 5, 7, 24, generator=g).cuda()
+    w, b = torch.randn(9, 24, 1, generator=g).cuda(), torch.randn(9, generator=g).cuda()
+    y = linear(x, w, b, act='relu')
+    assert y.shape == (2, 5, 7, 9) and torch.equal(y.reshape(-1, 9), linear(x.reshape(-1, 24), w[:, :, 0], b, act='relu'))
+    assert linear(x[0, 0, 0, :], w, b).shape == (9,)
+    assert linear(x[:0], w, b).shape == (0, 5, 7, 9) and layer_norm(x[:0]).shape == (0, 5, 7, 24)
+    for which in range(4):                                                  # one leaf at a time, the rest constants
+        t = [x.reshape(-1, 24).clone(), w[:, :, 0].clone(), b.clone(), torch.randn(70, 9, generator=g).cuda()]
+        full = [v.clone().requires_grad_() for v in t]
+        one = [v.requires_grad_() if i == which else v for i, v in enumerate(t)]
+        c = torch.randn(70, 9, generator=g).cuda()
+        for a in (full, one):
+            linear(a[0], a[1], a[2], act='silu', residual=a[3]).backward(c)
+        assert torch.equal(full[which].grad, one[which].grad)
+    # gradients that come as expanded or transposed tensors, and a zero-row batch
+    xg = torch.randn(33, 24, generator=g).cuda().requires_grad_()
+    wg = w[:, :, 0].clone().requires_grad_()
+    linear(xg, wg).sum().backward()
+    ref = torch.ones(33, 9, dtype=torch.float64)
+    close(xg.grad, ref @ wg.detach().cpu().double(), 1e-5, 'dx of a sum')
+    z = torch.zeros(0, 24, device='cuda', requires_grad=True)
+    wg.grad = None
+    bg = b.clone().requires_grad_()
+    linear(z, wg, bg, act='gelu').sum().backward()
+    assert z.grad.shape == (0, 24) and not bool(wg.grad.any()) and not bool(bg.grad.any())
+    gm = torch.ones(24, device='cuda', requires_grad=True)
+    layer_norm(z, gm).sum().backward()
+    assert not bool(gm.grad.any())
+    with pytest.raises(RuntimeError):                                       # no gradient of a gradient
+        q = torch.randn(4, 24, device='cuda', requires_grad=True)
+        (d,) = torch.autograd.grad(linear(q, wg, act='tanh').sum(), q, create_graph=True)
+        d.sum().backward()
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_the_same_bits_every_time_and_on_another_stream(dtype):
+    xd, x, w, b, r, dy = make(3000, 264, 200, dtype, residual=True)
+
+    def run():
+        leaves = [t.detach().clone().requires_grad_() for t in (xd, dev(w), dev(b))]
+        y = linear(leaves[0], leaves[1], leaves[2], act='gelu', residual=dev(r))
+        h = layer_norm(y, torch.ones(200, dtype=dtype, device='cuda', requires_grad=True))
+        return (y, h) + torch.autograd.grad(h, leaves, dy.cuda())
+    first = run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = run()
+    third = run()
+    torch.cuda.synchronize()
+    for a, c, d in zip(first, second, third):
+        assert torch.equal(a, c) and torch.equal(a, d)
+
+
+def test_captured_graphs_replay_with_new_inputs():
+    """Two graphs of a training step, captured one after the other, replayed in turn with eager work between: each keeps its own workspace."""
+    def step(x, w, b, dy):
+        y = linear(x, w, b, act='silu')
+        h = layer_norm(y)
+        return (h,) + torch.autograd.grad(h, (x, w, b), dy)
+    graphs = []
+    for m, k, n in ((1500, 136, 72), (40, 33, 65)):
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            static = [torch.randn(m, k, device='cuda').requires_grad_(), torch.randn(n, k, device='cuda').requires_grad_(), torch.randn(n, device='cuda').requires_grad_(),
+                      torch.randn(m, n, device='cuda')]
+            for _ in range(2):
+                step(*static)
+            torch.cuda.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                outs = step(*static)
+        graphs.append((g, static, outs, (m, k, n)))
+    for turn in range(3):
+        for g, static, outs, (m, k, n) in graphs:
+            with torch.no_grad():
+                for t in static:
+                    t.copy_(torch.randn(t.shape, device='cuda'))
+            g.replay()
+            torch.cuda.synchronize()
+            fresh = [t.detach().clone().requires_grad_() for t in static[:3]]
+            for a, c in zip(outs, step(*fresh, static[3])):
+                assert torch.equal(a, c)
+            torch.cuda.synchronize()
+
+
+def test_a_residual_block_as_it_is_used():
+    """x + W2 gelu(W1 norm(x) + b1) + b2 and its gradients, float32, against float64; relative to the largest value of each output 2e-5 (sums of 200 .. 900 float32 products)."""
+    g = torch.Generator().manual_seed(17)
+    t = [torch.randn(*s, generator=g) * f for s, f in (((900, 200), 1.0), ((200,), 0.3), ((200,), 0.1), ((560, 200), 200 ** -0.5), ((560,), 0.1), ((200, 560), 560 ** -0.5), ((200,), 0.1))]
+    dy = torch.randn(900, 200, generator=g)
+
+    def block(x, gm, bt, w1, b1, w2, b2, norm, lin):
+        return lin(lin(norm(x, gm, bt), w1, b1, 'gelu', None), w2, b2, None, x)
+    a = [v.cuda().requires_grad_() for v in t]
+    y = block(*a, norm=lambda x, gm, bt: layer_norm(x, gm, bt), lin=lambda x, w, b, act, r: linear(x, w, b, act=act, residual=r))
+    y.backward(dy.cuda())
+    d = [v.double().requires_grad_() for v in t]
+
+    def lin64(x, w, b, act, r):
+        z = x @ w.t() + b
+        z = z * 0.5 * torch.erfc(-z / math.sqrt(2)) if act else z
+        return z if r is None else z + r
+    ref = block(*d, norm=lambda x, gm, bt: torch.nn.functional.layer_norm(x, (200,), gm, bt), lin=lin64)
+    ref.backward(dy.double())
+    for got, want in [(y, ref)] + [(p.grad, q.grad) for p, q in zip(a, d)]:
+        close(got, want.detach(), 2e-5 * float(want.detach().abs().max()), 'block')
+
+
+@pytest.mark.parametrize('name', ['shared', 'geo', 'clr', 'recon'])
+def test_mlp_forward_is_the_network_s_own_stack(name):
+    """MLP.forward (any widths, layer by layer on linear) for the four stacks of the networks, with gradients, against the same stack of torch layers in float64 on the CPU."""
+    import golden_inputs as gi
+    from common import mlp_sd
+    from avatarcap_amd.network.mlp import MLP
+    kw = gi.MLP_CONFIGS[name]['kwargs']
+    net = MLP(**kw)
+    net.load_state_dict({k: torch.from_numpy(v) for k, v in mlp_sd(name).items()})
+    ref = MLP(**kw).double()
+    ref.load_state_dict({k: torch.from_numpy(v).double() for k, v in mlp_sd(name).items()})
+    net = net.cuda()
+    for B, N in ((1, 300), (2, 77), (1, 1)):
+        x = torch.randn(B, kw['in_channels'], N, generator=torch.Generator().manual_seed(B * 10 + N))
+        xd, xr = x.cuda().requires_grad_(), x.double().requires_grad_()
+        y = net(xd)
+        h = xr
+        last = len(ref.fc_list) - 1
+        for l, fc in enumerate(ref.fc_list):
+            conv = fc if l == last else fc[0]
+            if l in ref.res_layers:
+                h = torch.cat([h, xr], 1)
+            w = ref._weight(conv)
+            h = torch.einsum('oc,bcn->bon', w, h) + conv.bias[None, :, None]
+            act = ref.last_op if l == last else ref.nlactv
+            h = act64(h, act, 0.02)[0] if act not in ('relu', 'leaky_relu') else torch.where(h > 0, h, (0.02 if act == 'leaky_relu' else 0.0) * h)
+        assert y.shape == h.shape == (B, kw['out_channels'], N)
+        scale = float(h.detach().abs().max())
+        close(y, h.detach(), 2e-5 * max(scale, 1e-3), name)
+        c = torch.randn(h.shape, generator=torch.Generator().manual_seed(1))
+        net.zero_grad()
+        ref.zero_grad()
+        y.backward(c.cuda())
+        h.backward(c.double())
+        pairs = [(xd.grad, xr.grad)] + [(p.grad, dict(ref.named_parameters())[k].grad) for k, p in net.named_parameters()]
+        for got, want in pairs:
+            close(got, want, 1e-4 * float(want.abs().max()) + 1e-12, name)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('m,k,n', [(1, 3, 2), (17, 33, 65), (70, 9, 5), (130, 70, 131), (300, 520, 7)])
+def test_nothing_outside_of_the_outputs_is_written(m, k, n, dtype):
+    """The C entries on buffers between margins: inputs framed by NaNs, outputs by a pattern; row strides larger than the rows."""
+    L, ctx = _lib.lib(), _lib.ctx(0)
+    e = torch.finfo(dtype).bits // 8
+
+    class Box:
+        def __init__(self, rows, cols, fill=None, pad=3):
+            self.rows, self.cols, self.ld = rows, cols, cols + pad
+            self.raw = torch.full((1024 + rows * self.ld + 1024,), float('nan'), dtype=dtype, device='cuda')
+            self.v = self.raw[1024:1024 + rows * self.ld].view(rows, self.ld)[:, :cols]
+            if fill is not None:
+                self.v.copy_(fill)
+            self.ptr = self.raw.data_ptr() + 1024 * e
+
+        def outside_untouched(self):
+            mask = torch.ones_like(self.raw, dtype=torch.bool)
+            mask[1024:1024 + self.rows * self.ld].view(self.rows, self.ld)[:, :self.cols] = False
+            return bool(torch.isnan(self.raw[mask]).all()) and bool(torch.isfinite(self.v).all())
+    code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+    import ctypes as C
+    gen = torch.Generator().manual_seed(m + k + n)
+    x, w, b, r, dy = (Box(*s, fill=torch.randn(*s, generator=gen).to(dtype).cuda()) for s in ((m, k), (n, k), (1, n), (m, n), (m, n)))
+    y, z = Box(m, n), Box(m, n)
+    nb = C.c_int64()
+    _lib.check(L.avc_linear_workspace(m, n, k, code, x.ld, 1, C.byref(nb)))
+    ws = torch.empty(max(1, nb.value), dtype=torch.uint8, device='cuda')
+    _lib.check(L.avc_linear(ctx, x.ptr, x.ld, 1, w.ptr, w.ld, b.ptr, r.ptr, r.ld, 6, 0.0, m, n, k, code, y.ptr, y.ld, z.ptr, z.ld, ws.data_ptr(), nb.value, None))
+    torch.cuda.synchronize()
+    assert all(t.outside_untouched() for t in (x, w, b, r, y, z))
+    dx, dw, db = Box(m, k, pad=0), Box(n, k, pad=0), Box(1, n, pad=0)
+    _lib.check(L.avc_linear_backward_workspace(m, n, k, code, C.byref(nb)))
+    ws = torch.empty(max(1, nb.value), dtype=torch.uint8, device='cuda')
+    _lib.check(L.avc_linear_backward(ctx, dy.ptr, dy.ld, x.ptr, x.ld, 1, w.ptr, w.ld, z.ptr, z.ld, 6, 0.0, m, n, k, code, dx.ptr, dw.ptr, db.ptr, ws.data_ptr(), nb.value, None))
+    torch.cuda.synchronize()
+    assert all(t.outside_untouched() for t in (dx, dw, db))
+    y2, dx2, dg, dbt = Box(m, k), Box(m, k), Box(1, k), Box(1, k)
+    gm, dyk = Box(1, k, fill=torch.randn(1, k, generator=gen).to(dtype).cuda()), Box(m, k, fill=torch.randn(m, k, generator=gen).to(dtype).cuda())
+    st = torch.empty(2, m, device='cuda')
+    _lib.check(L.avc_layer_norm(ctx, x.ptr, x.ld, gm.ptr, None, 1e-5, m, k, code, y2.ptr, y2.ld, st[0].data_ptr(), st[1].data_ptr(), None))
+    _lib.check(L.avc_layer_norm_backward_workspace(m, k, code, C.byref(nb)))
+    ws = torch.empty(max(1, nb.value), dtype=torch.uint8, device='cuda')
+    _lib.check(L.avc_layer_norm_backward(ctx, dyk.ptr, dyk.ld, x.ptr, x.ld, gm.ptr, st[0].data_ptr(), st[1].data_ptr(), m, k, code, dx2.ptr, dx2.ld, dg.ptr, dbt.ptr, ws.data_ptr(), nb.value, None))
+    torch.cuda.synchronize()
+    assert all(t.outside_untouched() for t in (y2, dx2, dg, dbt))
+
+
+def test_in_place_outputs():
+    """y may be res itself (linear) or x itself (layer_norm) at the C entries."""
+    L, ctx = _lib.lib(), _lib.ctx(0)
+    g = torch.Generator().manual_seed(2)
+    for m, k, n in ((5, 40, 24), (300, 72, 136), (40, 4096, 64)):
+        x, w, r = (torch.randn(*s, generator=g).cuda() for s in ((m, k), (n, k), (m, n)))
+        want = linear(x, w, act='tanh', residual=r)
+        import ctypes as C
+        nb = C.c_int64()
+        _lib.check(L.avc_linear_workspace(m, n, k, 0, k, 1, C.byref(nb)))
+        ws = torch.empty(max(1, nb.value), dtype=torch.uint8, device='cuda')
+        _lib.check(L.avc_linear(ctx, x.data_ptr(), k, 1, w.data_ptr(), k, None, r.data_ptr(), n, 5, 0.0, m, n, k, 0, r.data_ptr(), n, None, 0, ws.data_ptr(), nb.value, None))
+        torch.cuda.synchronize()
+        assert torch.equal(r, want)
+    for m, c in ((7, 5), (33, 100), (9, 1023), (5, 9001), (3, 20001)):
+        x = torch.randn(m, c, generator=g).cuda()
+        want = layer_norm(x)
+        _lib.check(L.avc_layer_norm(ctx, x.data_ptr(), c, None, None, 1e-5, m, c, 0, x.data_ptr(), c, None, None, None))
+        torch.cuda.synchronize()
+        assert torch.equal(x, want)
+
+
+def test_the_current_device_stays_and_refusals_on_the_device():
+    x, w = torch.randn(4, 8, device='cuda'), torch.randn(3, 8, device='cuda')
+    before = torch.cuda.current_device()
+    linear(x, w)
+    assert torch.cuda.current_device() == before
+    with pytest.raises(TypeError):
+        linear(x, w.half())
+    with pytest.raises(TypeError):
+        linear(x.double(), w.double())
+    with pytest.raises(ValueError):
+        linear(x, w[:, :5])
+    with pytest.raises(ValueError):
+        linear(x, w, torch.randn(4, device='cuda'))
+    with pytest.raises(ValueError):
+        linear(x, w, residual=torch.randn(4, 4, device='cuda'))
+    with pytest.raises(ValueError):
+        linear(x, w, act='swish')
+    with pytest.raises(ValueError):
+        linear(x, w, act='leaky_relu', slope=-0.1)
+    with pytest.raises(RuntimeError):
+        linear(x, w.cpu())
+    with pytest.raises(ValueError):
+        layer_norm(x, torch.ones(7, device='cuda'))
+    with pytest.raises(ValueError):
+        layer_norm(x, eps=-1.0)
+    with pytest.raises(ValueError):
+        layer_norm(x[:, :0])
