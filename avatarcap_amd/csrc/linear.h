@@ -19,8 +19,8 @@ template <> struct Vec8<_Float16> { typedef f16x8 type; };
 template <> struct Vec8<float> { typedef f32x8 type; };
 
 // One operand of a product out(i, j) = sum_k P(i, k) Q(j, k).  `kc`: k is the contiguous axis and ld the distance of two rows; otherwise the rows are contiguous and ld is
-// the distance of two k.  Elements, not bytes.
-struct Operand { const void *p; int64_t ld; int kc; };
+// the distance of two k.  Elements, not bytes.  `padded`: 16-byte aligned rows whose last piece of 8 is there in full, zeros behind the end.
+struct Operand { const void *p; int64_t ld; int kc; int padded = 0; };
 
 struct Epilogue {
     const void *bias;                  // (N) or NULL
@@ -75,6 +75,34 @@ int layer_norm(const void *x, int64_t ldx, const void *g, const void *b, float e
 size_t layer_norm_backward_workspace(int64_t M, int64_t C, int dtype);
 int layer_norm_backward(const void *dy, int64_t lddy, const void *x, int64_t ldx, const void *g, const float *mean, const float *rstd, int64_t M, int64_t C, int dtype, void *dx, int64_t lddx,
                         void *dg, void *db, float *part, hipStream_t s);
+
+// x[j] <- x[j + s], zeros from the top; s = 0 .. 8
+__device__ __forceinline__ void shift_down(f32x8 &x, int s)
+{
+#pragma unroll
+    for (int b = 8; b >= 1; b >>= 1)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = s & b ? (j + b < 8 ? x[j + b < 8 ? j + b : j] : 0.f) : x[j];
+}
+__device__ __forceinline__ void shift_down(f32x4 &x, int s)                              // s = 0 .. 4
+{
+#pragma unroll
+    for (int b = 4; b >= 1; b >>= 1)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = s & b ? (j + b < 4 ? x[j + b < 4 ? j + b : j] : 0.f) : x[j];
+}
+template <typename X> __device__ __forceinline__ void shift_down(X &v, int s)             // 8 elements of 16 bits, two to a word
+{
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    u32x4 x = __builtin_bit_cast(u32x4, v);
+#pragma unroll
+    for (int b = 4; b >= 1; b >>= 1)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = s & (2 * b) ? (j + b < 4 ? x[j + b < 4 ? j + b : j] : 0u) : x[j];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = s & 1 ? (j < 3 ? __builtin_amdgcn_alignbit(x[j < 3 ? j + 1 : 3], x[j], 16) : x[j] >> 16) : x[j];
+    v = __builtin_bit_cast(X, x);
+}
 
 // ---- activations ------------------------------------------------------------------------------------------------------------------------------------------
 // float32 throughout, a few ulp each, from v_exp_f32 / v_rcp_f32: branch-free, so that an epilogue of tens of values per lane stays small.

@@ -215,33 +215,62 @@ template <typename T, int NB> __global__ __launch_bounds__(256) void narrow_kern
         }
 }
 
+// ---- runs of 16 bytes, whatever the alignment and the row's length -----------------------------------------------------------------------------------------------
+// The V values from column c on, zeros past the row's end.  A run that would pass the end is read further back, to end with the row, and shifted down: no lane branches
+// around a load.  Rows shorter than a run (SHORT) are read value by value.
+template <typename T> struct Run16 { static constexpr int V = 16 / sizeof(T); typedef T vec __attribute__((ext_vector_type(V))); };
+template <typename T, bool SHORT> __device__ __forceinline__ typename Run16<T>::vec read_run(const T *row, int64_t c, int64_t C)
+{
+    constexpr int V = Run16<T>::V;
+    typename Run16<T>::vec v;
+    if constexpr (SHORT) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = row[min(c + j, C - 1)];
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (c + j >= C) v[j] = (T)0.f;
+    } else {
+        const int64_t at = min(c, C - V);
+        __builtin_memcpy(&v, row + at, sizeof v);
+        shift_down(v, (int)min(c - at, (int64_t)V));
+    }
+    return v;
+}
+
 // ---- the activation's gradient dz = dy act'(z), and the column sums of dz in the same pass -------------------------------------------------------------------------
 // Lanes take V adjacent columns, `tx` lanes a row, 256 / tx rows at a time; every workgroup walks a strip of rows and leaves its column sums in part[strip][N] (float32, a
-// fixed order), which colsum_kernel adds (a single strip's sums are the bias gradient itself).  dz is rounded to the element type: it is the operand of two matrix products in that type.
-template <typename T, int V> __global__ __launch_bounds__(256) void dact_kernel(const T *__restrict__ dy, int64_t lddy, const T *__restrict__ z, int64_t ldz, int act, float slope, int64_t M, int64_t N,
-                                                                               int64_t rows_per, int tx, T *__restrict__ dz, float *__restrict__ part, T *__restrict__ db)
+// fixed order), which colsum_kernel adds (a single strip's sums are the bias gradient itself).  dz is rounded to the element type: it is the operand of two matrix products in
+// that type.  Its rows are padded with zeros to whole runs, so that the products read it in aligned pieces.  Bound by HBM: 4.9 TB/s at 65536 x 256 float32 (36 us).
+template <typename T, bool SHORT> __global__ __launch_bounds__(256) void dact_kernel(const T *__restrict__ dy, int64_t lddy, const T *__restrict__ z, int64_t ldz, int act, float slope, int64_t M,
+                                                                                    int64_t N, int64_t rows_per, int tx, T *__restrict__ dz, int64_t lddz, float *__restrict__ part,
+                                                                                    T *__restrict__ db)
 {
-    typedef T vec __attribute__((ext_vector_type(V)));
+    constexpr int V = Run16<T>::V;
+    typedef typename Run16<T>::vec vec;
     const int lx = threadIdx.x % tx, ly = threadIdx.x / tx, ty = 256 / tx;
     const int64_t n = ((int64_t)blockIdx.y * tx + lx) * V, m1 = min(M, ((int64_t)blockIdx.x + 1) * rows_per);
     float sum[V] = {};
     if (n < N) {
 #pragma unroll 2
         for (int64_t m = blockIdx.x * rows_per + ly; m < m1; m += ty) {
-            vec g = *reinterpret_cast<const vec *>(dy + m * lddy + n);
+            const vec g = read_run<T, SHORT>(dy + m * lddy, n, N);
             float v[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) v[j] = (float)g[j];
             if (z) {
-                const vec s = *reinterpret_cast<const vec *>(z + m * ldz + n);
-                vec o;
+                const vec s = read_run<T, SHORT>(z + m * ldz, n, N);
                 float zs[V], sl[V];
 #pragma unroll
                 for (int j = 0; j < V; ++j) zs[j] = (float)s[j];
                 slope_run<V>(zs, sl, act, slope);
 #pragma unroll
-                for (int j = 0; j < V; ++j) { v[j] *= sl[j]; o[j] = (T)v[j]; }
-                *reinterpret_cast<vec *>(dz + m * N + n) = o;
+                for (int j = 0; j < V; ++j) v[j] *= sl[j];
+            }
+            if (dz) {
+                vec o;
+#pragma unroll
+                for (int j = 0; j < V; ++j) o[j] = (T)v[j];
+                *reinterpret_cast<vec *>(dz + m * lddz + n) = o;
             }
 #pragma unroll
             for (int j = 0; j < V; ++j) sum[j] += v[j];
@@ -258,8 +287,21 @@ template <typename T, int V> __global__ __launch_bounds__(256) void dact_kernel(
         for (int j = 0; j < V; ++j) sum[j] += red[y * tx + lx][j];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
+        if (n + j >= N) continue;
         if (db) db[n + j] = (T)sum[j];
         else part[(int64_t)blockIdx.x * N + n + j] = sum[j];
+    }
+}
+
+// ---- rows copied to 16-byte aligned ones, zeros behind their ends ----------------------------------------------------------------------------------------------------
+template <typename T, bool SHORT> __global__ __launch_bounds__(256) void pad_kernel(const T *__restrict__ src, int64_t ld, int64_t R, int64_t C, T *__restrict__ dst, int64_t ldd)
+{
+    constexpr int V = Run16<T>::V;
+    const unsigned runs = (unsigned)(ldd / V);                          // below 2^22
+    const int64_t total = R * runs;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / runs, c = i % runs * V;
+        *reinterpret_cast<typename Run16<T>::vec *>(dst + r * ldd + c) = read_run<T, SHORT>(src + r * ld, c, C);
     }
 }
 
@@ -302,6 +344,7 @@ namespace {
 
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int esize(int dtype) { return dtype == AVC_F32 ? 4 : 2; }
+inline int64_t ceil8(int64_t n) { return (n + 7) & ~(int64_t)7; }
 
 // ---- which tile, how many splits: from the sizes alone, so that the workspace can be asked for in advance -----------------------------------------------------------
 // The time of a launch is estimated for every tile shape and a ladder of splits, and the least taken.  With W workgroups on the fullest CU, `occ` of them at a time, and S steps of
@@ -340,23 +383,39 @@ Plan plan_tiles(int64_t M, int64_t N, int64_t K, int dtype)
 }
 size_t partial_bytes(const Plan &p, int64_t M, int64_t N) { return p.splits > 1 ? sizeof(float) * (size_t)p.splits * (size_t)M * (size_t)N : 0; }
 
-// Large products whose last round of the large tile is mostly empty are cut: `rows` rows in full rounds, the rest in a launch of its own with the tile that suits it.  65537 rows of
-// 545 -> 256 float32 values need 514 tiles, three rounds of 256 for two rounds' work: 171 us; cut at 65536, 133 us.
-struct Cut { int64_t rows; Plan main, rest; };
+// A large product is cut where whole tiles or whole rounds of tiles end, if a main part of (rows, cols) and the strips below and to the right of it, each with the tile and splits
+// that suit it, come out cheaper than one launch whose last round or last row and column of tiles is mostly empty: 65537 rows of 545 -> 256 float32 values need 514 tiles, three
+// rounds of 256 for two rounds' work (171 us; cut at 65536, 133 us).
+struct Cut { int64_t rows, cols; Plan main, below, right; };
 Cut plan_cut(int64_t M, int64_t N, int64_t K, int dtype)
 {
-    Cut c{M, plan_tiles(M, N, K, dtype), Plan{}};
-    const int bm = tile_bm(dtype, TILE_BIG);
-    const int64_t tn = cdiv(N, tile_bn(dtype, TILE_BIG)), rounds = cdiv(M, bm) * tn / 256, rows = rounds * 256 / tn * bm;
-    if (rounds < 1 || rounds > 16 || rows < 1 || rows >= M || c.main.splits > 1) return c;
-    const Plan main = plan_tiles(rows, N, K, dtype), rest = plan_tiles(M - rows, N, K, dtype);
-    if (main.splits == 1 && main.us + rest.us + 3 < c.main.us) return Cut{rows, main, rest};
-    return c;
+    Cut best{M, N, plan_tiles(M, N, K, dtype), Plan{}, Plan{}};
+    double least = best.main.us;
+    const int64_t bm = tile_bm(dtype, TILE_BIG), bn = tile_bn(dtype, TILE_BIG);
+    if (least < 40 || best.main.splits > 1) return best;                // the strips are launches of their own
+    for (int64_t cols : {N, N / bn * bn}) {
+        if (cols < 1) continue;
+        const int64_t tn = cdiv(cols, bn), rounds = M / bm * tn / 256;
+        for (int64_t rows : {M, M / bm * bm, rounds >= 1 && rounds <= 16 ? rounds * 256 / tn * bm : (int64_t)0}) {
+            if (rows < 1 || rows > M || (rows == M && cols == N)) continue;
+            Cut c{rows, cols, plan_tiles(rows, cols, K, dtype), Plan{}, Plan{}};
+            if (c.main.splits > 1) continue;
+            double us = c.main.us;
+            if (rows < M) us += (c.below = plan_tiles(M - rows, cols, K, dtype)).us + 3;
+            if (cols < N) us += (c.right = plan_tiles(M, N - cols, K, dtype)).us + 3;
+            if (us < least) {
+                least = us;
+                best = c;
+            }
+        }
+    }
+    return best;
 }
 size_t product_bytes(int64_t M, int64_t N, int64_t K, int dtype)
 {
     const Cut c = plan_cut(M, N, K, dtype);
-    return std::max(partial_bytes(c.main, c.rows, N), c.rows < M ? partial_bytes(c.rest, M - c.rows, N) : 0);
+    return std::max(partial_bytes(c.main, c.rows, c.cols),
+                    std::max(c.rows < M ? partial_bytes(c.below, M - c.rows, c.cols) : 0, c.cols < N ? partial_bytes(c.right, M, N - c.cols) : 0));
 }
 
 // lanes that share a row in the activation-gradient pass
@@ -382,7 +441,7 @@ template <typename T> int launch_reduce(const float *part, int splits, int64_t M
     return AVC_OK;
 }
 
-int product_rows(const Operand &P, const Operand &Q, int64_t M, int64_t N, int64_t K, int dtype, const Epilogue &e, void *out, int64_t ldo, void *ws, const Plan &p, hipStream_t s)
+int product_part(const Operand &P, const Operand &Q, int64_t M, int64_t N, int64_t K, int dtype, const Epilogue &e, void *out, int64_t ldo, void *ws, const Plan &p, hipStream_t s)
 {
     AVC_REQUIRE((int64_t)p.tiles_m * p.tiles_n * p.splits < (1 << 22), AVC_ERR_ARG, "avc_linear: %lld x %lld outputs are more than one launch covers", (long long)M, (long long)N);
     TileArgs a{P, Q, M, N, K, out, ldo, e, (float *)ws, p.kper, p.tiles_m, p.tiles_n, p.splits};
@@ -395,17 +454,25 @@ int product_rows(const Operand &P, const Operand &Q, int64_t M, int64_t N, int64
 
 inline const void *ahead(const void *p, int64_t elements, int dtype) { return p ? (const char *)p + elements * esize(dtype) : nullptr; }
 
+// the operand, and the epilogue, from row m / column n of the output on
+Operand from(const Operand &o, int64_t row, int dtype) { return Operand{ahead(o.p, o.kc ? row * o.ld : row, dtype), o.ld, o.kc, o.padded}; }
+Epilogue from(const Epilogue &e, int64_t m, int64_t n, int dtype)
+{
+    return Epilogue{ahead(e.bias, n, dtype), ahead(e.res, m * e.ldr + n, dtype), e.ldr, (void *)ahead(e.z, m * e.ldz + n, dtype), e.ldz, e.act, e.slope};
+}
+
 int product(const Operand &P, const Operand &Q, int64_t M, int64_t N, int64_t K, int dtype, const Epilogue &e, void *out, int64_t ldo, void *ws, hipStream_t s)
 {
     const Cut c = plan_cut(M, N, K, dtype);
-    if (c.rows < M) {                                                    // the rows past the full rounds
-        const int64_t m = c.rows;
-        const Operand below{ahead(P.p, P.kc ? m * P.ld : m, dtype), P.ld, P.kc};
-        const Epilogue eb{e.bias, ahead(e.res, m * e.ldr, dtype), e.ldr, (void *)ahead(e.z, m * e.ldz, dtype), e.ldz, e.act, e.slope};
-        const int rc = product_rows(below, Q, M - m, N, K, dtype, eb, (void *)ahead(out, m * ldo, dtype), ldo, ws, c.rest, s);
+    if (c.rows < M) {
+        const int rc = product_part(from(P, c.rows, dtype), Q, M - c.rows, c.cols, K, dtype, from(e, c.rows, 0, dtype), (void *)ahead(out, c.rows * ldo, dtype), ldo, ws, c.below, s);
         if (rc != AVC_OK) return rc;
     }
-    return product_rows(P, Q, c.rows, N, K, dtype, e, out, ldo, ws, c.main, s);
+    if (c.cols < N) {
+        const int rc = product_part(P, from(Q, c.cols, dtype), M, N - c.cols, K, dtype, from(e, 0, c.cols, dtype), (void *)ahead(out, c.cols, dtype), ldo, ws, c.right, s);
+        if (rc != AVC_OK) return rc;
+    }
+    return product_part(P, Q, c.rows, c.cols, K, dtype, e, out, ldo, ws, c.main, s);
 }
 
 // ---- few rows ----------------------------------------------------------------------------------------------------------------------------------------------------
@@ -446,25 +513,55 @@ Route route(int64_t M, int64_t N, bool x_kc)
     return ROUTE_TILE;
 }
 
-template <typename T> int launch_dact(const void *dy, int64_t lddy, const void *z, int64_t ldz, int act, float slope, int64_t M, int64_t N, void *dz, float *part, void *db, int64_t strips, hipStream_t s)
+template <typename T> int launch_dact(const void *dy, int64_t lddy, const void *z, int64_t ldz, int act, float slope, int64_t M, int64_t N, void *dz, int64_t lddz, float *part, void *db,
+                                      int64_t strips, hipStream_t s)
 {
-    constexpr int V = 16 / sizeof(T);
-    const bool wide = N % V == 0 && lddy % V == 0 && ((uintptr_t)dy & 15) == 0 && (!z || (ldz % V == 0 && ((uintptr_t)z & 15) == 0));
-    const int v = wide ? V : 1;
-    const int tx = lanes_for(N, v);
-    const dim3 grid((unsigned)strips, (unsigned)cdiv(N, (int64_t)tx * v));
+    constexpr int V = Run16<T>::V;
+    const int tx = lanes_for(N, V);
+    const dim3 grid((unsigned)strips, (unsigned)cdiv(N, (int64_t)tx * V));
     const int64_t rows = cdiv(M, strips);
-    if (wide) hipLaunchKernelGGL((dact_kernel<T, V>), grid, dim3(256), 0, s, (const T *)dy, lddy, (const T *)z, ldz, act, slope, M, N, rows, tx, (T *)dz, part, (T *)db);
-    else hipLaunchKernelGGL((dact_kernel<T, 1>), grid, dim3(256), 0, s, (const T *)dy, lddy, (const T *)z, ldz, act, slope, M, N, rows, tx, (T *)dz, part, (T *)db);
+    if (N >= V) hipLaunchKernelGGL((dact_kernel<T, false>), grid, dim3(256), 0, s, (const T *)dy, lddy, (const T *)z, ldz, act, slope, M, N, rows, tx, (T *)dz, lddz, part, (T *)db);
+    else hipLaunchKernelGGL((dact_kernel<T, true>), grid, dim3(256), 0, s, (const T *)dy, lddy, (const T *)z, ldz, act, slope, M, N, rows, tx, (T *)dz, lddz, part, (T *)db);
     AVC_HIP(hipGetLastError());
     return AVC_OK;
+}
+
+// rows (R, C) of 16-bit elements copied to `dst` with rows of ceil8(C)
+int launch_pad(const Operand &o, int64_t R, int64_t C, void *dst, hipStream_t s)
+{
+    const int64_t ldd = ceil8(C), blocks = std::min<int64_t>(cdiv(R * (ldd / 8), 256), 1 << 16);
+    typedef __bf16 T;                                                   // bits are copied, whichever 16-bit type they are
+    if (C >= 8) hipLaunchKernelGGL((pad_kernel<T, false>), dim3((unsigned)blocks), dim3(256), 0, s, (const T *)o.p, o.ld, R, C, (T *)dst, ldd);
+    else hipLaunchKernelGGL((pad_kernel<T, true>), dim3((unsigned)blocks), dim3(256), 0, s, (const T *)o.p, o.ld, R, C, (T *)dst, ldd);
+    AVC_HIP(hipGetLastError());
+    return AVC_OK;
+}
+
+// 16-bit products whose operands' contiguous axes are no multiple of 8 cannot be read in direct pieces; staged through registers they take about twice as long (three times the weight
+// gradient).  Where copying the operands to padded rows costs less than 0.6 of the product, they are copied: 8191 x 2047 -> 2047 bf16, weight gradient 292 -> 126 us.
+// `elements` are those copied, `copies` the launches.
+bool worth_padding(double product_us, int64_t elements, int copies) { return elements && (double)elements * 4 / 4.5e6 + 3.0 * copies < 0.6 * product_us; }
+
+struct ForwardPad { bool x, w; size_t xb, wb, total; };
+ForwardPad forward_pad(int64_t M, int64_t N, int64_t K, int dtype, bool x_kc)
+{
+    ForwardPad f{};
+    if (dtype == AVC_F32) return f;
+    f.x = (x_kc ? K : M) % 8 != 0;
+    f.w = K % 8 != 0;
+    const int64_t xe = x_kc ? M * ceil8(K) : K * ceil8(M), we = N * ceil8(K);
+    if (!worth_padding(plan_cut(M, N, K, dtype).main.us, (f.x ? xe : 0) + (f.w ? we : 0), f.x + f.w)) return ForwardPad{};
+    f.xb = f.x ? align256((size_t)xe * 2) : 0;
+    f.wb = f.w ? align256((size_t)we * 2) : 0;
+    f.total = f.xb + f.wb;
+    return f;
 }
 
 }  // namespace
 
 size_t forward_workspace(int64_t M, int64_t N, int64_t K, int dtype, bool x_kc)
 {
-    return M && route(M, N, x_kc) == ROUTE_TILE ? product_bytes(M, N, K, dtype) : 0;
+    return M && route(M, N, x_kc) == ROUTE_TILE ? forward_pad(M, N, K, dtype, x_kc).total + product_bytes(M, N, K, dtype) : 0;
 }
 
 // Layers whose gradients are no more tiles than the chip has CUs, with sums of at most eight steps: the launches cost more than the work (20.6 us of host time and three launches
@@ -476,16 +573,26 @@ static bool small_backward(int64_t M, int64_t N, int64_t K, int dtype)
     return M >= 1 && M <= longest && N <= longest && cdiv(N, 64) * cdiv(K, 64) <= 256 && cdiv(M, 64) * cdiv(K, 64) <= 256;
 }
 
-struct BackwardSpace { size_t dz, strips, partial, total; };
+// The backward pass's workspace: dz (padded rows), the strips' column sums, padded copies of x and w, the splits' sums.  pad_dy: dy has no activation to pass and is copied as dz.
+struct BackwardSpace { size_t dz, strips, x, w, partial, total; bool pad_dy, pad_x, pad_w; };
 static BackwardSpace backward_space(int64_t M, int64_t N, int64_t K, int dtype)
 {
     BackwardSpace w{};
     if (small_backward(M, N, K, dtype)) return w;
-    w.dz = align256((size_t)M * N * esize(dtype));
+    const int64_t lddz = dtype == AVC_F32 ? (N + 3) & ~(int64_t)3 : ceil8(N);
+    w.dz = align256((size_t)M * lddz * esize(dtype));
     w.strips = align256(sizeof(float) * (size_t)strips_for(M, N, dtype) * N);
     w.partial = product_bytes(N, K, M, dtype);
     if (M) w.partial = std::max(w.partial, product_bytes(M, K, N, dtype));
-    w.total = w.dz + w.strips + w.partial;
+    if (dtype != AVC_F32 && M) {
+        const double us = plan_cut(M, K, N, dtype).main.us + 2 * plan_cut(N, K, M, dtype).main.us;
+        w.pad_dy = N % 8 != 0;
+        w.pad_x = w.pad_w = K % 8 != 0;                                 // (channel-first x is padded along M; the larger of the two is reserved)
+        const int64_t xe = std::max(M * ceil8(K), K * ceil8(M)), we = N * ceil8(K);
+        if (!worth_padding(us, (w.pad_dy ? M * ceil8(N) : 0) + (w.pad_x ? xe + we : 0), w.pad_dy + 2 * w.pad_x)) w.pad_dy = w.pad_x = w.pad_w = false;
+        if (w.pad_x) { w.x = align256((size_t)xe * 2); w.w = align256((size_t)we * 2); }
+    }
+    w.total = w.dz + w.strips + w.x + w.w + w.partial;
     return w;
 }
 size_t backward_workspace(int64_t M, int64_t N, int64_t K, int dtype) { return backward_space(M, N, K, dtype).total; }
@@ -496,8 +603,22 @@ int forward(const Operand &x, const void *w, int64_t ldw, int64_t M, int64_t N, 
     case ROUTE_FEW_ROWS: return AVC_BY_TYPE(dtype, launch_few)(w, ldw, N, x.p, x.ld, (int)M, K, 1, e, y, ldy, s);
     case ROUTE_FEW_COLS: return AVC_BY_TYPE(dtype, launch_few)(x.p, x.ld, M, w, ldw, (int)N, K, 0, e, y, ldy, s);
     case ROUTE_NARROW: return AVC_BY_TYPE(dtype, launch_narrow)(x.p, x.ld, w, ldw, M, (int)N, K, e, y, ldy, s);
-    default: return product(x, Operand{w, ldw, 1}, M, N, K, dtype, e, y, ldy, ws, s);
+    default: break;
     }
+    Operand P = x, Q{w, ldw, 1};
+    const ForwardPad f = forward_pad(M, N, K, dtype, x.kc);
+    char *space = (char *)ws;
+    if (f.x) {
+        const int rc = x.kc ? launch_pad(x, M, K, space, s) : launch_pad(x, K, M, space, s);
+        if (rc != AVC_OK) return rc;
+        P = Operand{space, x.kc ? ceil8(K) : ceil8(M), x.kc, 1};
+    }
+    if (f.w) {
+        const int rc = launch_pad(Q, N, K, space + f.xb, s);
+        if (rc != AVC_OK) return rc;
+        Q = Operand{space + f.xb, ceil8(K), 1, 1};
+    }
+    return product(P, Q, M, N, K, dtype, e, y, ldy, space + f.total, s);
 }
 
 int backward(const void *dy, int64_t lddy, const Operand &x, const void *w, int64_t ldw, const void *z, int64_t ldz, int act, float slope, int64_t M, int64_t N, int64_t K, int dtype,
@@ -517,11 +638,12 @@ int backward(const void *dy, int64_t lddy, const Operand &x, const void *w, int6
         return dtype == AVC_F32 ? launch_small_f32(a, (unsigned)blocks, x.kc, s) : dtype == AVC_BF16 ? launch_small_bf16(a, (unsigned)blocks, x.kc, s) : launch_small_f16(a, (unsigned)blocks, x.kc, s);
     }
     const BackwardSpace sp = backward_space(M, N, K, dtype);
-    char *dz_buf = (char *)ws, *strips_buf = dz_buf + sp.dz, *part = strips_buf + sp.strips;
-    const bool active = act != AVC_ACT_NONE;
-    if (active || db) {
+    char *dz_buf = (char *)ws, *strips_buf = dz_buf + sp.dz, *x_buf = strips_buf + sp.strips, *w_buf = x_buf + sp.x, *part = w_buf + sp.w;
+    const bool active = act != AVC_ACT_NONE, through = active || sp.pad_dy;      // dz is dy itself, or goes through the pass below
+    const int64_t lddz = through ? (dtype == AVC_F32 ? (N + 3) & ~(int64_t)3 : ceil8(N)) : lddy;
+    if (through || db) {
         const int64_t strips = strips_for(M, N, dtype);
-        const int rc = AVC_BY_TYPE(dtype, launch_dact)(dy, lddy, active ? z : nullptr, ldz, act, slope, M, N, dz_buf, db && strips > 1 ? (float *)strips_buf : nullptr,
+        const int rc = AVC_BY_TYPE(dtype, launch_dact)(dy, lddy, active ? z : nullptr, ldz, act, slope, M, N, through ? dz_buf : nullptr, lddz, db && strips > 1 ? (float *)strips_buf : nullptr,
                                                        strips == 1 ? db : nullptr, strips, s);
         if (rc != AVC_OK) return rc;
         if (db && strips > 1) {
@@ -529,14 +651,25 @@ int backward(const void *dy, int64_t lddy, const Operand &x, const void *w, int6
             if (rc2 != AVC_OK) return rc2;
         }
     }
-    const void *dz = active ? dz_buf : dy;
-    const int64_t lddz = active ? N : lddy;
+    const void *dz = through ? dz_buf : dy;
     if (dx && M) {
-        const int rc = product(Operand{dz, lddz, 1}, Operand{w, ldw, 0}, M, K, N, dtype, none, dx, K, part, s);
+        Operand Q{w, ldw, 0};
+        if (sp.pad_w) {
+            const int rc = launch_pad(Q, N, K, w_buf, s);
+            if (rc != AVC_OK) return rc;
+            Q = Operand{w_buf, ceil8(K), 0, 1};
+        }
+        const int rc = product(Operand{dz, lddz, 1, through}, Q, M, K, N, dtype, none, dx, K, part, s);
         if (rc != AVC_OK) return rc;
     }
     if (dw) {
-        const int rc = product(Operand{dz, lddz, 0}, Operand{x.p, x.ld, x.kc ? 0 : 1}, N, K, M, dtype, none, dw, K, part, s);
+        Operand Q{x.p, x.ld, x.kc ? 0 : 1};
+        if (sp.pad_x && (x.kc || M % 8)) {
+            const int rc = x.kc ? launch_pad(x, M, K, x_buf, s) : launch_pad(x, K, M, x_buf, s);
+            if (rc != AVC_OK) return rc;
+            Q = Operand{x_buf, x.kc ? ceil8(K) : ceil8(M), x.kc ? 0 : 1, 1};
+        }
+        const int rc = product(Operand{dz, lddz, 0, through}, Q, N, K, M, dtype, none, dw, K, part, s);
         if (rc != AVC_OK) return rc;
     }
     return AVC_OK;

@@ -98,7 +98,7 @@ template <int BR, bool KC> struct Tile {
 };
 
 // ---- global -> LDS ------------------------------------------------------------------------------------------------------------------------------------------
-// (a) direct: 16-byte pieces straight into LDS.  The host has checked that every piece lies wholly inside or outside of the operand and is 16-byte aligned; pieces outside get an
+// (a) direct: 16-byte pieces straight into LDS.  The host has checked that every piece lies wholly inside or outside of the operand (or of its padding) and is 16-byte aligned; pieces outside get an
 //     offset past the buffer's end, for which the hardware writes zeros.
 constexpr unsigned OUTSIDE = 0x80000000u;
 
@@ -113,7 +113,8 @@ template <int BR, bool KC, int NW> struct Direct {
     __device__ __forceinline__ void init(const Operand &o, int64_t row0, int64_t rows, int64_t k0, int64_t K, int wave, int lane)
     {
         ld_bytes = o.ld * 2;
-        const int64_t first = KC ? row0 * o.ld + k0 : k0 * o.ld + row0, last = KC ? (rows - 1) * o.ld + K : (K - 1) * o.ld + rows;
+        // (the contiguous axis is a multiple of 8, or padded to one)
+        const int64_t first = KC ? row0 * o.ld + k0 : k0 * o.ld + row0, last = KC ? (rows - 1) * o.ld + ((K + 7) & ~(int64_t)7) : (K - 1) * o.ld + ((rows + 7) & ~(int64_t)7);
         base = (const char *)o.p + first * 2;
         left = (last - first) * 2;
         step_bytes = KC ? BK * 2 : BK * ld_bytes;
@@ -157,27 +158,6 @@ template <typename X> __device__ __forceinline__ void split3(const X &x, bf16x8 
         out[1][j] = m;
         out[2][j] = (__bf16)(r - (float)m);
     }
-}
-
-// x[j] <- x[j + s], zeros from the top; s = 0 .. 8
-__device__ __forceinline__ void shift_down(f32x8 &x, int s)
-{
-#pragma unroll
-    for (int b = 8; b >= 1; b >>= 1)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = s & b ? (j + b < 8 ? x[j + b < 8 ? j + b : j] : 0.f) : x[j];
-}
-template <typename X> __device__ __forceinline__ void shift_down(X &v, int s)             // 16-bit elements, two to a word
-{
-    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-    u32x4 x = __builtin_bit_cast(u32x4, v);
-#pragma unroll
-    for (int b = 4; b >= 1; b >>= 1)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = s & (2 * b) ? (j + b < 4 ? x[j + b < 4 ? j + b : j] : 0u) : x[j];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = s & 1 ? (j < 3 ? __builtin_amdgcn_alignbit(x[j < 3 ? j + 1 : 3], x[j], 16) : x[j] >> 16) : x[j];
-    v = __builtin_bit_cast(X, x);
 }
 
 template <int BR, bool KC, int NT> struct Staged {
@@ -352,19 +332,17 @@ template <int READS, int MFMAS> __device__ __forceinline__ void interleave()
     }
 }
 
-template <int VEC> __device__ __forceinline__ void store_run(elem_t *dst, const float *v, int64_t left, bool vec)
+// 16 bytes of a row, of any alignment; what passes the row's end is left out
+template <int VEC> __device__ __forceinline__ void store_run(elem_t *dst, const float *v, int64_t left)
 {
-    if (vec && left >= VEC) {
-        typedef elem_t ev __attribute__((ext_vector_type(VEC)));
-        ev o;
+    elem_t o[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) o[j] = (elem_t)v[j];
-        *reinterpret_cast<ev *>(dst) = o;
-    } else {
+    for (int j = 0; j < VEC; ++j) o[j] = (elem_t)v[j];
+    if (left >= VEC) __builtin_memcpy(dst, o, sizeof o);
+    else
 #pragma unroll
         for (int j = 0; j < VEC; ++j)
-            if (j < left) dst[j] = (elem_t)v[j];
-    }
+            if (j < left) dst[j] = o[j];
 }
 
 // Steps of LDS.  float32's middle tile keeps one (48 KB), so that three workgroups share a CU and fill each other's waits; everything else two.
@@ -478,7 +456,6 @@ __device__ __forceinline__ void tile_body(const TileArgs &a, const Slope &dz, un
     const int64_t mw = m0 + pr0, nw = n0 + qr0;                         // the wave's corner
     if (a.splits > 1) {
         float *part = a.partial + (int64_t)split * a.M * a.N;
-        const bool vec = (a.N & 3) == 0;
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
             const int64_t m = mw + 16 * i + (lane & 15);
@@ -487,7 +464,7 @@ __device__ __forceinline__ void tile_body(const TileArgs &a, const Slope &dz, un
             for (int f = 0; f < FN; ++f) {
                 const int64_t n = nw + 16 * f + 4 * (lane >> 4);
                 float *dst = part + m * a.N + n;
-                if (vec && n + 4 <= a.N) *reinterpret_cast<f32x4 *>(dst) = acc[i][f];
+                if (n + 4 <= a.N) __builtin_memcpy(dst, &acc[i][f], 16);
                 else
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
@@ -500,8 +477,6 @@ __device__ __forceinline__ void tile_body(const TileArgs &a, const Slope &dz, un
     static_assert(NW * 32 * PITCH <= STAGES * STAGE, "the epilogue's rows do not fit LDS");
     typedef elem_t run_t __attribute__((ext_vector_type(VEC)));
     const Epilogue &e = a.ep;
-    const bool vec_out = (a.ldo % VEC) == 0 && ((uintptr_t)a.out & 15) == 0, vec_z = (e.ldz % VEC) == 0 && ((uintptr_t)e.z & 15) == 0,
-               vec_res = (e.ldr % VEC) == 0 && ((uintptr_t)e.res & 15) == 0;
     const int col = lane % LPR * VEC;
     const int64_t n = nw + col, left = a.N - n;
     float bias[VEC];
@@ -525,7 +500,7 @@ __device__ __forceinline__ void tile_body(const TileArgs &a, const Slope &dz, un
             res[it] = run_t(0);
             if (e.res && m < a.M && left > 0) {
                 const elem_t *r = (const elem_t *)e.res + m * e.ldr + n;
-                if (vec_res && left >= VEC) res[it] = *reinterpret_cast<const run_t *>(r);
+                if (left >= VEC) __builtin_memcpy(&res[it], r, sizeof res[it]);
                 else
 #pragma unroll
                     for (int j = 0; j < VEC; ++j)
@@ -544,12 +519,12 @@ __device__ __forceinline__ void tile_body(const TileArgs &a, const Slope &dz, un
                 for (int k = 0; k < 4; ++k) v[j + k] = x[k] + bias[j + k];
             }
             if (m >= a.M || left <= 0) continue;
-            if (e.z) store_run<VEC>((elem_t *)e.z + m * e.ldz + n, v, left, vec_z);
+            if (e.z) store_run<VEC>((elem_t *)e.z + m * e.ldz + n, v, left);
             act_run<VEC>(v, e.act, e.slope);
             if (e.res)
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) v[j] += (float)res[it][j];
-            store_run<VEC>((elem_t *)a.out + m * a.ldo + n, v, left, vec_out);
+            store_run<VEC>((elem_t *)a.out + m * a.ldo + n, v, left);
         }
         __builtin_amdgcn_wave_barrier();
     }
@@ -648,7 +623,7 @@ template <bool XKC> int launch_small(const SmallArgs &a, unsigned blocks, hipStr
 bool direct_ok(const Operand &o, int64_t rows, int64_t K)
 {
     const int64_t inner = o.kc ? K : rows;
-    return ((uintptr_t)o.p & 15) == 0 && o.ld % 8 == 0 && inner % 8 == 0 && o.ld < (int64_t)1 << 21;
+    return ((uintptr_t)o.p & 15) == 0 && o.ld % 8 == 0 && (o.padded || inner % 8 == 0) && o.ld < (int64_t)1 << 21;
 }
 
 }  // namespace
