@@ -28,18 +28,21 @@ template <int V> struct Run {
 
 template <int V, typename T> __device__ __forceinline__ void load_run(const T *row, int64_t at, float *out)
 {
-    T v[V];
-    __builtin_memcpy(v, row + at, sizeof v);
+    typedef T vec __attribute__((ext_vector_type(V)));
+    typedef vec loose __attribute__((aligned(sizeof(T))));               // one load, whatever the alignment
+    const vec v = *reinterpret_cast<const loose *>(row + at);
 #pragma unroll
     for (int j = 0; j < V; ++j) out[j] = (float)v[j];
 }
 
 template <int V, typename T> __device__ __forceinline__ void store_run(T *row, const Run<V> &run, const float *in)
 {
-    T v[V];
+    typedef T vec __attribute__((ext_vector_type(V)));
+    typedef vec loose __attribute__((aligned(sizeof(T))));
+    vec v;
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = (T)in[j];
-    if (run.first == 0) __builtin_memcpy(row + run.at, v, sizeof v);
+    if (run.first == 0) *reinterpret_cast<loose *>(row + run.at) = v;
     else
 #pragma unroll
         for (int j = 1; j < V; ++j)

@@ -271,6 +271,7 @@ template <typename T, bool SHORT> __global__ __launch_bounds__(256) void dact_ke
 #pragma unroll
                 for (int j = 0; j < V; ++j) o[j] = (T)v[j];
                 *reinterpret_cast<vec *>(dz + m * lddz + n) = o;
+                if (V < 8 && n + V >= N && n + V < lddz) *reinterpret_cast<vec *>(dz + m * lddz + n + V) = vec(0);      // float32: rows of 8, runs of 4
             }
 #pragma unroll
             for (int j = 0; j < V; ++j) sum[j] += v[j];
@@ -392,7 +393,7 @@ Cut plan_cut(int64_t M, int64_t N, int64_t K, int dtype)
     Cut best{M, N, plan_tiles(M, N, K, dtype), Plan{}, Plan{}};
     double least = best.main.us;
     const int64_t bm = tile_bm(dtype, TILE_BIG), bn = tile_bn(dtype, TILE_BIG);
-    if (least < 40 || best.main.splits > 1) return best;                // the strips are launches of their own
+    if (least < 40) return best;                                        // the strips are launches of their own
     for (int64_t cols : {N, N / bn * bn}) {
         if (cols < 1) continue;
         const int64_t tn = cdiv(cols, bn), rounds = M / bm * tn / 256;
@@ -526,33 +527,41 @@ template <typename T> int launch_dact(const void *dy, int64_t lddy, const void *
     return AVC_OK;
 }
 
-// rows (R, C) of 16-bit elements copied to `dst` with rows of ceil8(C)
-int launch_pad(const Operand &o, int64_t R, int64_t C, void *dst, hipStream_t s)
+// rows (R, C) copied to `dst` with rows of ceil8(C)
+template <typename T> int launch_pad_as(const Operand &o, int64_t R, int64_t C, void *dst, hipStream_t s)
 {
-    const int64_t ldd = ceil8(C), blocks = std::min<int64_t>(cdiv(R * (ldd / 8), 256), 1 << 16);
-    typedef __bf16 T;                                                   // bits are copied, whichever 16-bit type they are
-    if (C >= 8) hipLaunchKernelGGL((pad_kernel<T, false>), dim3((unsigned)blocks), dim3(256), 0, s, (const T *)o.p, o.ld, R, C, (T *)dst, ldd);
+    constexpr int V = Run16<T>::V;
+    const int64_t ldd = ceil8(C), blocks = std::min<int64_t>(cdiv(R * (ldd / V), 256), 1 << 16);
+    if (C >= V) hipLaunchKernelGGL((pad_kernel<T, false>), dim3((unsigned)blocks), dim3(256), 0, s, (const T *)o.p, o.ld, R, C, (T *)dst, ldd);
     else hipLaunchKernelGGL((pad_kernel<T, true>), dim3((unsigned)blocks), dim3(256), 0, s, (const T *)o.p, o.ld, R, C, (T *)dst, ldd);
     AVC_HIP(hipGetLastError());
     return AVC_OK;
 }
+int launch_pad(const Operand &o, int64_t R, int64_t C, int dtype, void *dst, hipStream_t s)          // 16 bits are copied as bits, whichever type they are
+{
+    return dtype == AVC_F32 ? launch_pad_as<float>(o, R, C, dst, s) : launch_pad_as<__bf16>(o, R, C, dst, s);
+}
 
 // 16-bit products whose operands' contiguous axes are no multiple of 8 cannot be read in direct pieces; staged through registers they take about twice as long (three times the weight
-// gradient).  Where copying the operands to padded rows costs less than 0.6 of the product, they are copied: 8191 x 2047 -> 2047 bf16, weight gradient 292 -> 126 us.
+// gradient).  Where copying the operands to padded rows costs less than 0.6 of the product, they are copied: 8191 x 2047 -> 2047 bf16, forward 120 -> 89 us, weight gradient
+// 292 -> 118 us.  Not for short calls (`least`, us): a host that cannot run ahead pays for every launch (16387 x 319 -> 256 float16 training: 126 us without copies, 132 with).
+// float32 is staged in any case, but the workgroups at a ragged edge of rows that lie contiguously shift every piece they read and hold up the rest: worth 0.3 of the product there.
 // `elements` are those copied, `copies` the launches.
-bool worth_padding(double product_us, int64_t elements, int copies) { return elements && (double)elements * 4 / 4.5e6 + 3.0 * copies < 0.6 * product_us; }
+bool worth_padding(double product_us, double least, int64_t elements, int copies, int dtype)
+{
+    return elements && product_us >= least && (double)elements * 2 * esize(dtype) / 4.5e6 + 3.0 * copies < (dtype == AVC_F32 ? 0.3 : 0.6) * product_us;
+}
 
 struct ForwardPad { bool x, w; size_t xb, wb, total; };
 ForwardPad forward_pad(int64_t M, int64_t N, int64_t K, int dtype, bool x_kc)
 {
     ForwardPad f{};
-    if (dtype == AVC_F32) return f;
-    f.x = (x_kc ? K : M) % 8 != 0;
-    f.w = K % 8 != 0;
+    f.x = x_kc ? dtype != AVC_F32 && K % 8 != 0 : M % 8 != 0;
+    f.w = dtype != AVC_F32 && K % 8 != 0;
     const int64_t xe = x_kc ? M * ceil8(K) : K * ceil8(M), we = N * ceil8(K);
-    if (!worth_padding(plan_cut(M, N, K, dtype).main.us, (f.x ? xe : 0) + (f.w ? we : 0), f.x + f.w)) return ForwardPad{};
-    f.xb = f.x ? align256((size_t)xe * 2) : 0;
-    f.wb = f.w ? align256((size_t)we * 2) : 0;
+    if (!worth_padding(plan_cut(M, N, K, dtype).main.us, 30, (f.x ? xe : 0) + (f.w ? we : 0), f.x + f.w, dtype)) return ForwardPad{};
+    f.xb = f.x ? align256((size_t)xe * esize(dtype)) : 0;
+    f.wb = f.w ? align256((size_t)we * esize(dtype)) : 0;
     f.total = f.xb + f.wb;
     return f;
 }
@@ -579,18 +588,18 @@ static BackwardSpace backward_space(int64_t M, int64_t N, int64_t K, int dtype)
 {
     BackwardSpace w{};
     if (small_backward(M, N, K, dtype)) return w;
-    const int64_t lddz = dtype == AVC_F32 ? (N + 3) & ~(int64_t)3 : ceil8(N);
+    const int64_t lddz = ceil8(N);
     w.dz = align256((size_t)M * lddz * esize(dtype));
     w.strips = align256(sizeof(float) * (size_t)strips_for(M, N, dtype) * N);
     w.partial = product_bytes(N, K, M, dtype);
     if (M) w.partial = std::max(w.partial, product_bytes(M, K, N, dtype));
-    if (dtype != AVC_F32 && M) {
+    if (M) {
         const double us = plan_cut(M, K, N, dtype).main.us + 2 * plan_cut(N, K, M, dtype).main.us;
         w.pad_dy = N % 8 != 0;
         w.pad_x = w.pad_w = K % 8 != 0;                                 // (channel-first x is padded along M; the larger of the two is reserved)
         const int64_t xe = std::max(M * ceil8(K), K * ceil8(M)), we = N * ceil8(K);
-        if (!worth_padding(us, (w.pad_dy ? M * ceil8(N) : 0) + (w.pad_x ? xe + we : 0), w.pad_dy + 2 * w.pad_x)) w.pad_dy = w.pad_x = w.pad_w = false;
-        if (w.pad_x) { w.x = align256((size_t)xe * 2); w.w = align256((size_t)we * 2); }
+        if (!worth_padding(us, 60, (w.pad_dy ? M * ceil8(N) : 0) + (w.pad_x ? xe + we : 0), w.pad_dy + 2 * w.pad_x, dtype)) w.pad_dy = w.pad_x = w.pad_w = false;
+        if (w.pad_x) { w.x = align256((size_t)xe * esize(dtype)); w.w = align256((size_t)we * esize(dtype)); }
     }
     w.total = w.dz + w.strips + w.x + w.w + w.partial;
     return w;
@@ -609,12 +618,12 @@ int forward(const Operand &x, const void *w, int64_t ldw, int64_t M, int64_t N, 
     const ForwardPad f = forward_pad(M, N, K, dtype, x.kc);
     char *space = (char *)ws;
     if (f.x) {
-        const int rc = x.kc ? launch_pad(x, M, K, space, s) : launch_pad(x, K, M, space, s);
+        const int rc = x.kc ? launch_pad(x, M, K, dtype, space, s) : launch_pad(x, K, M, dtype, space, s);
         if (rc != AVC_OK) return rc;
         P = Operand{space, x.kc ? ceil8(K) : ceil8(M), x.kc, 1};
     }
     if (f.w) {
-        const int rc = launch_pad(Q, N, K, space + f.xb, s);
+        const int rc = launch_pad(Q, N, K, dtype, space + f.xb, s);
         if (rc != AVC_OK) return rc;
         Q = Operand{space + f.xb, ceil8(K), 1, 1};
     }
@@ -640,7 +649,7 @@ int backward(const void *dy, int64_t lddy, const Operand &x, const void *w, int6
     const BackwardSpace sp = backward_space(M, N, K, dtype);
     char *dz_buf = (char *)ws, *strips_buf = dz_buf + sp.dz, *x_buf = strips_buf + sp.strips, *w_buf = x_buf + sp.x, *part = w_buf + sp.w;
     const bool active = act != AVC_ACT_NONE, through = active || sp.pad_dy;      // dz is dy itself, or goes through the pass below
-    const int64_t lddz = through ? (dtype == AVC_F32 ? (N + 3) & ~(int64_t)3 : ceil8(N)) : lddy;
+    const int64_t lddz = through ? ceil8(N) : lddy;
     if (through || db) {
         const int64_t strips = strips_for(M, N, dtype);
         const int rc = AVC_BY_TYPE(dtype, launch_dact)(dy, lddy, active ? z : nullptr, ldz, act, slope, M, N, through ? dz_buf : nullptr, lddz, db && strips > 1 ? (float *)strips_buf : nullptr,
@@ -655,7 +664,7 @@ int backward(const void *dy, int64_t lddy, const Operand &x, const void *w, int6
     if (dx && M) {
         Operand Q{w, ldw, 0};
         if (sp.pad_w) {
-            const int rc = launch_pad(Q, N, K, w_buf, s);
+            const int rc = launch_pad(Q, N, K, dtype, w_buf, s);
             if (rc != AVC_OK) return rc;
             Q = Operand{w_buf, ceil8(K), 0, 1};
         }
@@ -665,7 +674,7 @@ int backward(const void *dy, int64_t lddy, const Operand &x, const void *w, int6
     if (dw) {
         Operand Q{x.p, x.ld, x.kc ? 0 : 1};
         if (sp.pad_x && (x.kc || M % 8)) {
-            const int rc = x.kc ? launch_pad(x, M, K, x_buf, s) : launch_pad(x, K, M, x_buf, s);
+            const int rc = x.kc ? launch_pad(x, M, K, dtype, x_buf, s) : launch_pad(x, K, M, dtype, x_buf, s);
             if (rc != AVC_OK) return rc;
             Q = Operand{x_buf, x.kc ? ceil8(K) : ceil8(M), x.kc ? 0 : 1, 1};
         }

@@ -170,6 +170,7 @@ template <int BR, bool KC, int NT> struct Staged {
     int64_t ld, rows, axis;                                             // bytes; rows left from row0 on; length of the contiguous axis
     __device__ __forceinline__ void init(const Operand &o, int64_t row0, int64_t nrows, int64_t k0, int64_t K, int tid)
     {
+        if (!KC && o.padded) nrows = (nrows + 7) & ~(int64_t)7;         // the padding is read as rows of zeros
         axis = KC ? K : nrows;
         ld = o.ld * (int64_t)sizeof(elem_t);
         rows = nrows - row0;
@@ -332,13 +333,15 @@ template <int READS, int MFMAS> __device__ __forceinline__ void interleave()
     }
 }
 
-// 16 bytes of a row, of any alignment; what passes the row's end is left out
+// 16 bytes of a row, of any alignment; what passes the row's end is left out.  (One store of a vector type: of a copy from an array the compiler makes several.)
 template <int VEC> __device__ __forceinline__ void store_run(elem_t *dst, const float *v, int64_t left)
 {
-    elem_t o[VEC];
+    typedef elem_t vec __attribute__((ext_vector_type(VEC)));
+    typedef vec loose __attribute__((aligned(sizeof(elem_t))));
+    vec o;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) o[j] = (elem_t)v[j];
-    if (left >= VEC) __builtin_memcpy(dst, o, sizeof o);
+    if (left >= VEC) *reinterpret_cast<loose *>(dst) = o;
     else
 #pragma unroll
         for (int j = 0; j < VEC; ++j)
@@ -455,6 +458,7 @@ __device__ __forceinline__ void tile_body(const TileArgs &a, const Slope &dz, un
     // ---- epilogue
     const int64_t mw = m0 + pr0, nw = n0 + qr0;                         // the wave's corner
     if (a.splits > 1) {
+        typedef f32x4 loose4 __attribute__((aligned(4)));
         float *part = a.partial + (int64_t)split * a.M * a.N;
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
@@ -464,7 +468,7 @@ __device__ __forceinline__ void tile_body(const TileArgs &a, const Slope &dz, un
             for (int f = 0; f < FN; ++f) {
                 const int64_t n = nw + 16 * f + 4 * (lane >> 4);
                 float *dst = part + m * a.N + n;
-                if (n + 4 <= a.N) __builtin_memcpy(dst, &acc[i][f], 16);
+                if (n + 4 <= a.N) *reinterpret_cast<loose4 *>(dst) = acc[i][f];
                 else
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
@@ -476,6 +480,7 @@ __device__ __forceinline__ void tile_body(const TileArgs &a, const Slope &dz, un
     constexpr int VEC = 16 / sizeof(elem_t), WCOLS = BN / WN, PITCH = WCOLS * 4 + 16, LPR = WCOLS / VEC, RPI = 64 / LPR, ITER = 32 / RPI;
     static_assert(NW * 32 * PITCH <= STAGES * STAGE, "the epilogue's rows do not fit LDS");
     typedef elem_t run_t __attribute__((ext_vector_type(VEC)));
+    typedef run_t loose_t __attribute__((aligned(sizeof(elem_t))));
     const Epilogue &e = a.ep;
     const int col = lane % LPR * VEC;
     const int64_t n = nw + col, left = a.N - n;
@@ -500,7 +505,7 @@ __device__ __forceinline__ void tile_body(const TileArgs &a, const Slope &dz, un
             res[it] = run_t(0);
             if (e.res && m < a.M && left > 0) {
                 const elem_t *r = (const elem_t *)e.res + m * e.ldr + n;
-                if (left >= VEC) __builtin_memcpy(&res[it], r, sizeof res[it]);
+                if (left >= VEC) res[it] = *reinterpret_cast<const loose_t *>(r);
                 else
 #pragma unroll
                     for (int j = 0; j < VEC; ++j)

@@ -584,3 +584,40 @@ def test_the_current_device_stays_and_refusals_on_the_device():
         layer_norm(x, eps=-1.0)
     with pytest.raises(ValueError):
         layer_norm(x[:, :0])
+
+
+def test_offsets_past_32_bits():
+    """Matrices of more than 2^32 bytes and 2^31 elements: the last rows of the large call against a small call on them, to half a step of the type (their sums may be ordered otherwise)."""
+    m, k, n = 9_000_001, 256, 240
+    x = torch.empty(m, k, dtype=torch.bfloat16, device='cuda')
+    x[:] = torch.randn(1, k, device='cuda')
+    tail = torch.randn(700, k, device='cuda').to(x.dtype)
+    x[-700:] = tail
+    w, b = (torch.randn(n, k, device='cuda') / 16).to(x.dtype).requires_grad_(), torch.randn(n, device='cuda').to(x.dtype).requires_grad_()
+    y = linear(x, w, b, act='relu')
+    assert y.numel() > 2 ** 31
+    close(y[-700:].detach(), dbl(linear(tail, w, b, act='relu')), 2 * unit(x.dtype) * dbl(y[-700:]).abs() + 1e-6, 'last rows')
+    # a gradient in which the last rows alone count
+    dy = torch.zeros(m, n, dtype=x.dtype, device='cuda')
+    dy[-700:] = torch.randn(700, n, device='cuda').to(x.dtype)
+    dw, db = torch.autograd.grad(y, (w, b), dy)
+    t = tail.clone().requires_grad_()
+    w2, b2 = w.detach().clone().requires_grad_(), b.detach().clone().requires_grad_()
+    dt2, dw2, db2 = torch.autograd.grad(linear(t, w2, b2, act='relu'), (t, w2, b2), dy[-700:].contiguous())
+    for got, want in ((dw, dw2), (db, db2)):
+        close(got, dbl(want), 2 * unit(x.dtype) * dbl(want).abs() + 1e-4 * float(want.abs().max()), 'gradients')
+    del dy, y
+    h = layer_norm(x)
+    close(h[-700:], dbl(layer_norm(tail)), 2 * unit(x.dtype) * dbl(h[-700:]).abs() + 1e-6, 'norm of the last rows')
+    del h
+    xt = torch.empty(k, m, dtype=torch.bfloat16, device='cuda')              # channel-first points, their rows 18 MB apart
+    xt[:] = x.t()
+    y1 = linear(xt.t(), w.detach()[:1])
+    close(y1[-700:], dbl(linear(tail, w.detach()[:1])), 2 * unit(x.dtype) * dbl(y1[-700:]).abs() + 1e-2 * 2.0 ** -8, 'one output')
+    y2 = linear(xt.t(), w.detach()[:40])
+    close(y2[-700:], dbl(linear(tail, w.detach()[:40])), 2 * unit(x.dtype) * dbl(y2[-700:]).abs() + 1e-2 * 2.0 ** -8, 'forty outputs')
+    wl = w.detach()[:5].clone().requires_grad_()
+    out = linear(xt.t(), wl)
+    (dw5,) = torch.autograd.grad(out, wl, torch.cat([torch.zeros(m - 700, 5, device='cuda', dtype=x.dtype), torch.ones(700, 5, device='cuda', dtype=x.dtype)]))
+    want = dbl(tail).sum(0).expand(5, k)
+    close(dw5, want, 2 * unit(x.dtype) * want.abs() + 700 * E32 * dbl(tail).abs().sum(0), 'weight gradient of channel-first points')
