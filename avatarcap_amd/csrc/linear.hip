@@ -14,7 +14,7 @@ template <typename T> __device__ __forceinline__ void finish(float v, int64_t m,
     if (e.bias) v += (float)((const T *)e.bias)[n];
     if (e.z) ((T *)e.z)[m * e.ldz + n] = (T)v;
     float a[1] = {v};
-    act_run<1>(a, e.act, e.slope);
+    act_run<sizeof(T) == 2, 1>(a, e.act, e.slope);
     v = a[0];
     if (e.res) v += (float)((const T *)e.res)[m * e.ldr + n];
     out[m * ldo + n] = (T)v;
@@ -146,7 +146,7 @@ template <typename T, int FB> __global__ __launch_bounds__(1024) void few_kernel
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (a.ep.z && mine && s0 + 4 * q + j < a.ns) ((T *)a.ep.z)[m[j] * a.ep.ldz + n[j]] = (T)v[j];
-        act_run<4>(v, a.ep.act, a.ep.slope);
+        act_run<sizeof(T) == 2, 4>(v, a.ep.act, a.ep.slope);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (mine && s0 + 4 * q + j < a.ns) a.out[m[j] * a.ldo + n[j]] = (T)(a.ep.res ? v[j] + res[j] : v[j]);
@@ -262,7 +262,7 @@ template <typename T, bool SHORT> __global__ __launch_bounds__(256) void dact_ke
                 float zs[V], sl[V];
 #pragma unroll
                 for (int j = 0; j < V; ++j) zs[j] = (float)s[j];
-                slope_run<V>(zs, sl, act, slope);
+                slope_run<sizeof(T) == 2, V>(zs, sl, act, slope);
 #pragma unroll
                 for (int j = 0; j < V; ++j) v[j] *= sl[j];
             }

@@ -273,7 +273,7 @@ template <int BR, bool KC, int NT> struct StagedSlope {
                 float zs[8], sl[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) zs[j] = (float)z.v[i][j];
-                slope_run<8>(zs, sl, act, slope);
+                slope_run<!IS_F32, 8>(zs, sl, act, slope);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] = (elem_t)((float)x[j] * sl[j]);
             }
@@ -525,7 +525,7 @@ __device__ __forceinline__ void tile_body(const TileArgs &a, const Slope &dz, un
             }
             if (m >= a.M || left <= 0) continue;
             if (e.z) store_run<VEC>((elem_t *)e.z + m * e.ldz + n, v, left);
-            act_run<VEC>(v, e.act, e.slope);
+            act_run<!IS_F32, VEC>(v, e.act, e.slope);
             if (e.res)
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) v[j] += (float)res[it][j];
@@ -566,7 +566,7 @@ template <bool XKC> __global__ __launch_bounds__(256, 2) void small_backward_ker
                 g[j] = (float)dy[r * a.lddy];
                 zs[j] = a.act != AVC_ACT_NONE ? (float)z[r * a.ld_saved] : 0.f;
             }
-            slope_run<4>(zs, sl, a.act, a.slope);
+            slope_run<!IS_F32, 4>(zs, sl, a.act, a.slope);
 #pragma unroll
             for (int j = 0; j < 4; ++j) s += m + 16 * j < a.M ? g[j] * sl[j] : 0.f;
         }
