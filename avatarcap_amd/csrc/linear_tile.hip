@@ -125,7 +125,16 @@ template <int BR, bool KC, int NW> struct Direct {
             if (KC ? row0 + r >= rows : row0 + p * 8 >= rows) voff[i] = OUTSIDE;
         }
     }
-    // the pieces of the step that starts at the current base, `kleft` values of k from it on
+    // the pieces of a whole step that starts at the current base
+    __device__ __forceinline__ void issue_whole(char *lds, int wave)
+    {
+        __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)min(left, (int64_t)0x7fffffff), 0x00020000);
+#pragma unroll
+        for (int i = 0; i < N; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void *)(lds + (i * NW + wave) * 1024), 16, (int)voff[i], 0, 0, 0);
+        base += step_bytes;
+        left -= step_bytes;
+    }
+    // the same where `kleft` values of k may end the step
     __device__ __forceinline__ void issue(char *lds, int64_t kleft, int wave, int lane)
     {
         __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)min(left, (int64_t)0x7fffffff), 0x00020000);
@@ -322,14 +331,19 @@ template <int FM, int FN> __device__ __forceinline__ void multiply(const half8 (
 #pragma unroll
         for (int t = 0; t < FN; ++t) acc[i][t] = mfma(q[t], p[i], acc[i][t]);
 }
-// deals READS LDS reads evenly among MFMAS matrix instructions of the surrounding block
-template <int READS, int MFMAS> __device__ __forceinline__ void interleave()
+// deals READS LDS reads, and behind them LOADS loads into LDS, evenly among MFMAS matrix instructions of the surrounding block
+template <int READS, int MFMAS, int LOADS> __device__ __forceinline__ void interleave()
 {
-    constexpr int PER = MFMAS / READS > 0 ? MFMAS / READS : 1;
+    constexpr int PER = (MFMAS - LOADS) / READS > 0 ? (MFMAS - LOADS) / READS : 1;
 #pragma unroll
     for (int i = 0; i < READS; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
     }
 }
 
@@ -407,17 +421,19 @@ __device__ __forceinline__ void tile_body(const TileArgs &a, const Slope &dz, un
             half8 p0[FM], q0[FN], p1[FM], q1[FN];
             read_fragments<FN, LQ>(q0, smem + LP::BYTES, rq, 0);
             read_fragments<FM, LP>(p0, smem, rp, 0);
-            for (int s = 0; s < steps; ++s) {
+            // WHOLE: step s + 2 exists and is whole, so that its loads need no branch and can be dealt among the matrix instructions like the LDS reads
+            auto step = [&](int s, auto whole) {
+                constexpr bool WHOLE = decltype(whole)::value;
                 char *cur = smem + (s & 1) * STAGE, *nxt = smem + ((s + 1) & 1) * STAGE;
                 read_fragments<FN, LQ>(q1, cur + LP::BYTES, rq, 1);
                 read_fragments<FM, LP>(p1, cur, rp, 1);
                 multiply(p0, q0, acc);
-                interleave<READS, FM * FN>();
+                interleave<READS, FM * FN, 0>();
                 __builtin_amdgcn_sched_barrier(0);
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
                 __builtin_amdgcn_s_barrier();
                 asm volatile("" ::: "memory");
-                if (s + 2 < steps) {
+                if (!WHOLE && s + 2 < steps) {
                     const int64_t kleft = kend - k0 - (int64_t)(s + 2) * BK;
                     dp.issue(cur, kleft, wave, lane);
                     dq.issue(cur + LP::BYTES, kleft, wave, lane);
@@ -425,10 +441,18 @@ __device__ __forceinline__ void tile_body(const TileArgs &a, const Slope &dz, un
                 // (the last step reads what the other buffer holds and uses none of it)
                 read_fragments<FN, LQ>(q0, nxt + LP::BYTES, rq, 0);
                 read_fragments<FM, LP>(p0, nxt, rp, 0);
+                if constexpr (WHOLE) {
+                    dp.issue_whole(cur, wave);
+                    dq.issue_whole(cur + LP::BYTES, wave);
+                }
                 multiply(p1, q1, acc);
-                interleave<READS, FM * FN>();
+                interleave<READS, FM * FN, WHOLE ? Direct<BM, PKC, NW>::N + Direct<BN, QKC, NW>::N : 0>();
                 __builtin_amdgcn_sched_barrier(0);
-            }
+            };
+            const int whole = (int)((kend - k0) / BK) - 2;
+            int s = 0;
+            for (; s < whole; ++s) step(s, std::true_type{});
+            for (; s < steps; ++s) step(s, std::false_type{});
         }
     } else {
         typename std::conditional<DZ, StagedSlope<BM, PKC, NT>, Staged<BM, PKC, NT>>::type sp;
