@@ -187,6 +187,9 @@ template <bool HALF, int V> __device__ __forceinline__ void act_run(float (&v)[V
     }
 }
 
+// +-infinity as a large finite value, for slopes that multiply z with what has long become 0: a float16 z beyond 65504 is stored as infinity while its y and gradient are finite
+__device__ __forceinline__ float finite(float z) { return fabsf(z) == __builtin_inff() ? copysignf(1e15f, z) : z; }
+
 // v[j] = act'(z[j]).  For the two piecewise linear ones the sign is all that counts, so that z may be the activation's value.
 template <bool HALF, int V> __device__ __forceinline__ void slope_run(const float (&zs)[V], float (&v)[V], int act, float slope)
 {
@@ -202,8 +205,8 @@ template <bool HALF, int V> __device__ __forceinline__ void slope_run(const floa
     case AVC_ACT_SOFTPLUS: AVC_RUN(z > 20.f ? 1.f : sigmoid_of<HALF>(z, u))
     case AVC_ACT_SIGMOID: AVC_RUN((e = sigmoid_of<HALF>(z, u), e * u))
     case AVC_ACT_TANH: AVC_RUN((e = sigmoid_of<HALF>(2.f * z, u), 4.f * e * u))
-    case AVC_ACT_GELU: AVC_RUN((u = normal_tail<HALF>(z, e), fmaf(z * 0.3989422804014327f, e, z >= 0.f ? 1.f - u : u)))
-    case AVC_ACT_SILU: AVC_RUN((e = sigmoid_of<HALF>(z, u), e * fmaf(z, u, 1.f)))
+    case AVC_ACT_GELU: AVC_RUN((u = normal_tail<HALF>(z, e), fmaf(finite(z) * 0.3989422804014327f, e, z >= 0.f ? 1.f - u : u)))
+    case AVC_ACT_SILU: AVC_RUN((e = sigmoid_of<HALF>(z, u), e * fmaf(finite(z), u, 1.f)))
     default: AVC_RUN(1.f)
     }
 #undef AVC_RUN

@@ -412,8 +412,10 @@ Cut plan_cut(int64_t M, int64_t N, int64_t K, int dtype)
     }
     return best;
 }
+constexpr int64_t MOST_ROWS = (int64_t)1 << 26;                          // per launch; products of more rows are cut into blocks of this many
 size_t product_bytes(int64_t M, int64_t N, int64_t K, int dtype)
 {
+    if (M > MOST_ROWS) return std::max(product_bytes(MOST_ROWS, N, K, dtype), M % MOST_ROWS ? product_bytes(M % MOST_ROWS, N, K, dtype) : 0);
     const Cut c = plan_cut(M, N, K, dtype);
     return std::max(partial_bytes(c.main, c.rows, c.cols),
                     std::max(c.rows < M ? partial_bytes(c.below, M - c.rows, c.cols) : 0, c.cols < N ? partial_bytes(c.right, M, N - c.cols) : 0));
@@ -464,6 +466,13 @@ Epilogue from(const Epilogue &e, int64_t m, int64_t n, int dtype)
 
 int product(const Operand &P, const Operand &Q, int64_t M, int64_t N, int64_t K, int dtype, const Epilogue &e, void *out, int64_t ldo, void *ws, hipStream_t s)
 {
+    if (M > MOST_ROWS) {
+        for (int64_t m = 0; m < M; m += MOST_ROWS) {
+            const int rc = product(from(P, m, dtype), Q, std::min(MOST_ROWS, M - m), N, K, dtype, from(e, m, 0, dtype), (void *)ahead(out, m * ldo, dtype), ldo, ws, s);
+            if (rc != AVC_OK) return rc;
+        }
+        return AVC_OK;
+    }
     const Cut c = plan_cut(M, N, K, dtype);
     if (c.rows < M) {
         const int rc = product_part(from(P, c.rows, dtype), Q, M - c.rows, c.cols, K, dtype, from(e, c.rows, 0, dtype), (void *)ahead(out, c.rows * ldo, dtype), ldo, ws, c.below, s);

@@ -168,8 +168,9 @@ def linear(x, weight, bias=None, act=None, slope=0.02, residual=None):
     slope = float(slope)
     if act == 'leaky_relu' and not 0.0 <= slope < float('inf'):
         raise ValueError(f'linear: leaky_relu takes a finite slope >= 0, got {slope}')
-    x2 = x if x.dim() == 2 else x.reshape(-1, k)
-    r2 = None if residual is None else _rows(residual if residual.dim() == 2 else residual.reshape(-1, n))
+    m = x.numel() // k
+    x2 = x if x.dim() == 2 else x.reshape(m, k)
+    r2 = None if residual is None else _rows(residual if residual.dim() == 2 else residual.reshape(m, n))
     if bias is not None and n > 1 and bias.stride(0) != 1:
         bias = bias.contiguous()
     code = ACTS[act]
@@ -227,7 +228,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     eps = float(eps)
     if not 0.0 <= eps < float('inf'):
         raise ValueError(f'layer_norm: eps must be finite and >= 0, got {eps}')
-    x2 = x if x.dim() == 2 else x.reshape(-1, c)
+    x2 = x if x.dim() == 2 else x.reshape(x.numel() // c, c)
     weight, bias = (t if t is None or c == 1 or t.stride(0) == 1 else t.contiguous() for t in (weight, bias))
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
         y = _LayerNorm.apply(x2, weight, bias, eps)

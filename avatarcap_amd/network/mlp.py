@@ -50,7 +50,7 @@ class MLP(nn.Module):
         if x.dim() != 3 or x.shape[1] != self.all_channels[0]:
             raise ValueError(f'MLP: expected (B, {self.all_channels[0]}, N), got {tuple(x.shape)}')
         B, _, N = x.shape
-        x0 = x[0].t() if B == 1 else x.transpose(1, 2).reshape(B * N, -1)      # points as rows; for one batch entry a view that the kernels read as it lies
+        x0 = x[0].t() if B == 1 else x.transpose(1, 2).reshape(B * N, self.all_channels[0])      # points as rows; for one batch entry a view that the kernels read as it lies
         h = x0
         last = len(self.fc_list) - 1
         for l, fc in enumerate(self.fc_list):
@@ -58,7 +58,7 @@ class MLP(nn.Module):
             if l in self.res_layers:
                 h = torch.cat([h, x0], dim=1)
             h = linear(h, self._weight(conv), conv.bias, act=self.last_op if l == last else self.nlactv)
-        return h.reshape(B, N, -1).transpose(1, 2).contiguous()
+        return h.reshape(B, N, self.all_channels[-1]).transpose(1, 2).contiguous()
 
 
 class OffsetDecoder(nn.Module):

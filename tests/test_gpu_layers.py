@@ -621,3 +621,58 @@ def test_offsets_past_32_bits():
     (dw5,) = torch.autograd.grad(out, wl, torch.cat([torch.zeros(m - 700, 5, device='cuda', dtype=x.dtype), torch.ones(700, 5, device='cuda', dtype=x.dtype)]))
     want = dbl(tail).sum(0).expand(5, k)
     close(dw5, want, 2 * unit(x.dtype) * want.abs() + 700 * E32 * dbl(tail).abs().sum(0), 'weight gradient of channel-first points')
+
+
+def test_slopes_where_float16_overflows():
+    """z = +-80000 is infinite in float16 while gelu and silu, and their slopes, are 0 or z and 1: the gradient stays finite."""
+    for act in ('gelu', 'silu', 'tanh', 'sigmoid', 'soft_plus'):
+        x = torch.tensor([[-400.0], [400.0]], dtype=torch.float16, device='cuda')
+        w = torch.tensor([[200.0]], dtype=torch.float16, device='cuda').requires_grad_()
+        y = linear(x, w, act=act)
+        (g,) = torch.autograd.grad(y, w, torch.tensor([[1.0], [0.0]], dtype=torch.float16, device='cuda'))
+        assert float(y[0, 0].abs()) <= 1 and float(g) == 0.0, (act, y, g)
+
+
+def test_more_rows_than_a_launch_takes():
+    m, k, n = (1 << 26) + 77, 8, 24
+    x = torch.randn(1, k, device='cuda').to(torch.bfloat16).expand(m, k).contiguous()
+    x[-400:] = torch.randn(400, k, device='cuda').to(x.dtype)
+    w = torch.randn(n, k, device='cuda').to(x.dtype).requires_grad_()
+    y = linear(x, w, act='relu')
+    assert torch.equal(y[-400:], linear(x[-400:].contiguous(), w, act='relu')) and torch.equal(y[:1].expand(5, n), y[12345:12350])
+    dy = torch.zeros_like(y)
+    dy[-400:] = 1
+    (dw,) = torch.autograd.grad(y, w, dy)
+    want = ((dbl(x[-400:]) @ dbl(w).t() > 0).double().t() @ dbl(x[-400:]))
+    kink = (dbl(x[-400:]) @ dbl(w).t()).abs() < 1e-5
+    assert not bool(kink.any())
+    close(dw, want, 2 * unit(x.dtype) * want.abs() + 400 * E32 * dbl(x[-400:]).abs().sum(0), 'dw')
+
+
+def test_empty_batches_of_the_mlp():
+    from avatarcap_amd.network.mlp import MLP
+    net = MLP(6, 2, [16, 8], res_layers=[1]).cuda()
+    for shape in ((1, 6, 0), (0, 6, 5), (2, 6, 0)):
+        assert net(torch.zeros(shape, device='cuda')).shape == (shape[0], 2, shape[2])
+    with pytest.raises(ValueError):
+        net(torch.zeros(1, 5, 4, device='cuda'))
+    with pytest.raises(TypeError):
+        net(torch.zeros(1, 6, 4, device='cuda').half())
+    half = net.half()
+    assert half(torch.ones(1, 6, 4, device='cuda').half()).dtype == torch.float16
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('layout', ['rows', 'channels'])
+def test_padded_copies_and_cuts(layout, dtype):
+    """Odd sizes large enough that operands are copied to padded rows and the product is cut into a main part and strips (the workspace says so)."""
+    import ctypes as C
+    m, k, n = 4099, 1027, 2055
+    nb = C.c_int64()
+    code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+    xr, xc = (k, 1) if layout == 'rows' else (1, m)
+    _lib.check(_lib.lib().avc_linear_workspace(m, n, k, code, xr, xc, C.byref(nb)))
+    copied = (k + 5) * m * (4 if code == 0 else 2)
+    assert nb.value >= (0 if code == 0 and layout == 'rows' else copied * 0.99)
+    check_linear(m, k, n, dtype, act='silu', layout=layout, residual=True)
+    check_linear(m, k, n, dtype, layout=layout, bias=False)
