@@ -20,18 +20,6 @@ template <typename T> __device__ __forceinline__ void finish(float v, int64_t m,
     out[m * ldo + n] = (T)v;
 }
 
-// ---- sums of the splits: one thread per output value, the splits added in order ----------------------------------------------------------------------------------
-template <typename T> __global__ __launch_bounds__(256) void reduce_kernel(const float *__restrict__ part, int splits, int64_t M, int64_t N, T *out, int64_t ldo, const Epilogue e)
-{
-    const int64_t total = M * N;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        float v = 0.f;
-#pragma unroll 8
-        for (int s = 0; s < splits; ++s) v += part[s * total + i];
-        finish<T>(v, i / N, i % N, e, out, ldo);
-    }
-}
-
 // ---- few rows: out(f, s) = sum_k F(f, k) S(s, k) with at most 16 * FB rows f against a long operand S that is read once -------------------------------------------
 // A wave takes 16 rows of S and all rows of F on 16-row matrix instructions; the k axis is dealt in chunks of 128 bytes per row to the workgroup's waves, whose sums meet in
 // LDS.  Lane (row l, quarter q) loads 32 adjacent bytes of its row, so a row's chunk is one 128-byte line.  float32 uses the f32 matrix instruction: the call is bound by the
@@ -311,11 +299,11 @@ template <typename T, bool SHORT> __global__ __launch_bounds__(256) void pad_ker
 // out(n) = sum over the strips of part[strip][n]: 32 columns and 32 runs of strips per workgroup, the runs' sums added in order.  Columns past N1 belong to the second output.
 // A few hundred strips of a few hundred columns are too few bytes to matter; what counts is the chain of dependent loads, so 1024 threads share it (8 runs took 38 - 74 us for
 // 1024 - 2048 strips).
-template <typename T> __global__ __launch_bounds__(1024) void colsum_kernel(const float *__restrict__ part, int strips, int64_t N, int64_t N1, T *out, T *out2)
+template <typename T> __device__ __forceinline__ void column_sums(const float *__restrict__ part, int strips, int64_t N, int64_t N1, T *out, T *out2, unsigned block)
 {
     __shared__ float red[32][33];
     const int lx = threadIdx.x & 31, ly = threadIdx.x >> 5;
-    const int64_t n = (int64_t)blockIdx.x * 32 + lx;
+    const int64_t n = (int64_t)block * 32 + lx;
     float s = 0.f;
     if (n < N) {
 #pragma unroll 8
@@ -328,6 +316,59 @@ template <typename T> __global__ __launch_bounds__(1024) void colsum_kernel(cons
     for (int y = 1; y < 32; ++y) s += red[y][lx];
     if (n < N1) { if (out) out[n] = (T)s; }
     else if (out2) out2[n - N1] = (T)s;
+}
+template <typename T> __global__ __launch_bounds__(1024) void colsum_kernel(const float *__restrict__ part, int strips, int64_t N, int64_t N1, T *out, T *out2)
+{
+    column_sums<T>(part, strips, N, N1, out, out2, blockIdx.x);
+}
+
+// ---- sums of the splits, added in order: four adjacent outputs per thread where there are many (24 -> 12 us for 2 x 2048 x 2048), one where there are few (128 x 256 x 256: 11 us,
+// 23 us with four).  The workgroups past `blocks` take the bias gradient's column sums along, a launch saved.
+constexpr int64_t SMALL_REDUCE = 1 << 20;
+template <typename T> __global__ __launch_bounds__(1024) void reduce_kernel(const float *__restrict__ part, int splits, int64_t M, int64_t N, T *out, int64_t ldo, const Epilogue e, unsigned blocks,
+                                                                            const float *__restrict__ strip_part, int strips, int64_t columns, T *sums)
+{
+    if (blockIdx.x >= blocks) {
+        column_sums<T>(strip_part, strips, columns, columns, sums, (T *)nullptr, blockIdx.x - blocks);
+        return;
+    }
+    const int64_t total = M * N, stride = (int64_t)blocks * 1024;
+    if (total < SMALL_REDUCE || N % 4) {
+        for (int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x; i < total; i += stride) {
+            float v = 0.f;
+#pragma unroll 8
+            for (int s = 0; s < splits; ++s) v += part[s * total + i];
+            finish<T>(v, i / N, i % N, e, out, ldo);
+        }
+        return;
+    }
+    const bool small = total <= 0xffffffffll;                           // uniform; a 64-bit division costs more than the loads
+    typedef T vec __attribute__((ext_vector_type(4)));
+    typedef vec loose __attribute__((aligned(sizeof(T))));
+    for (int64_t i = 4 * ((int64_t)blockIdx.x * 1024 + threadIdx.x); i < total; i += 4 * stride) {
+        f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+        for (int s = 0; s < splits; ++s) a += *reinterpret_cast<const f32x4 *>(part + s * total + i);
+        const int64_t m = small ? (int64_t)((unsigned)i / (unsigned)N) : i / N, n = i - m * N;
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = a[j] + (e.bias ? (float)((const T *)e.bias)[n + j] : 0.f);
+        vec o;
+        if (e.z) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = (T)v[j];
+            *reinterpret_cast<loose *>((T *)e.z + m * e.ldz + n) = o;
+        }
+        act_run<sizeof(T) == 2, 4>(v, e.act, e.slope);
+        if (e.res) {
+            const vec r = *reinterpret_cast<const loose *>((const T *)e.res + m * e.ldr + n);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] += (float)r[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = (T)v[j];
+        *reinterpret_cast<loose *>(out + m * ldo + n) = o;
+    }
 }
 
 static int launch_columns(const float *part, int strips, int64_t N, int64_t N1, int dtype, void *out, void *out2, hipStream_t s)
@@ -351,11 +392,11 @@ inline int64_t ceil8(int64_t n) { return (n + 7) & ~(int64_t)7; }
 // The time of a launch is estimated for every tile shape and a ladder of splits, and the least taken.  With W workgroups on the fullest CU, `occ` of them at a time, and S steps of
 // k each:   launch + max(ceil(W / occ) (S lone_step + lone), W (S step + rest)) + the splits' sums written, read and reduced.
 // `lone_*` is a workgroup's own latency, `step` / `rest` its share of a busy CU (matrix rate; writing the tile out).  Constants in us, fitted to 1020 timed launches of 17 shapes
-// (64 .. 262144 rows, 64 .. 4096 columns and k, all three products): the choice came out 2 % slower than the best of all tiles and splits in the mean, 63 % at worst (64 -> 1024
-// float32 on 33000 rows, 77 us for 48).
+// (64 .. 262144 rows, 64 .. 4096 columns and k, all three products): the choice came out 2 % slower than the best of all tiles and splits in the mean, 44 % at worst (2048 x 2048
+// -> 512 bf16, 19 us for 13).
 struct TileCost { int occ; double lone_step, lone, step, rest; };
-constexpr TileCost COST_16[3] = {{1, 1.61, 6.9, 0.20, 11.2}, {2, 0.88, 2.1, 0.46, 3.2}, {5, 0.61, 0.0, 0.20, 1.0}};
-constexpr TileCost COST_F32[3] = {{1, 1.99, 6.9, 2.75, 3.6}, {3, 2.80, 3.1, 1.62, 3.1}, {3, 0.92, 1.8, 0.58, 1.0}};
+constexpr TileCost COST_16[3] = {{1, 1.28, 8.3, 0.91, 0.0}, {2, 0.76, 2.8, 0.43, 3.0}, {5, 0.52, 0.0, 0.18, 1.0}};
+constexpr TileCost COST_F32[3] = {{1, 2.74, 4.3, 0.00, 10.9}, {3, 2.82, 2.4, 1.60, 2.5}, {3, 0.90, 1.7, 0.57, 1.0}};
 constexpr int SPLITS[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256};
 
 struct Plan { int tile, tiles_m, tiles_n, splits; int64_t kper; double us; };
@@ -436,23 +477,29 @@ int64_t strips_for(int64_t M, int64_t N, int dtype)
 }
 
 inline size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
-template <typename T> int launch_reduce(const float *part, int splits, int64_t M, int64_t N, void *out, int64_t ldo, const Epilogue &e, hipStream_t s)
+// column sums that wait for a launch to join: out = NULL once they have
+struct Sums { const float *part; int strips; int64_t N; void *out; };
+
+template <typename T> int launch_reduce(const float *part, int splits, int64_t M, int64_t N, void *out, int64_t ldo, const Epilogue &e, Sums *sums, hipStream_t s)
 {
-    const int64_t blocks = std::min<int64_t>(cdiv(M * N, 256), 8192);
-    hipLaunchKernelGGL(reduce_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, part, splits, M, N, (T *)out, ldo, e);
+    const unsigned blocks = (unsigned)std::min<int64_t>(cdiv(M * N, M * N < SMALL_REDUCE || N % 4 ? 1024 : 4096), 8192), more = sums && sums->out ? (unsigned)cdiv(sums->N, 32) : 0;
+    hipLaunchKernelGGL(reduce_kernel<T>, dim3(blocks + more), dim3(1024), 0, s, part, splits, M, N, (T *)out, ldo, e, blocks, more ? sums->part : nullptr, more ? sums->strips : 0,
+                       more ? sums->N : 0, more ? (T *)sums->out : nullptr);
     AVC_HIP(hipGetLastError());
+    if (more) sums->out = nullptr;
     return AVC_OK;
 }
 
-int product_part(const Operand &P, const Operand &Q, int64_t M, int64_t N, int64_t K, int dtype, const Epilogue &e, void *out, int64_t ldo, void *ws, const Plan &p, hipStream_t s)
+int product_part(const Operand &P, const Operand &Q, int64_t M, int64_t N, int64_t K, int dtype, const Epilogue &e, void *out, int64_t ldo, void *ws, const Plan &p, hipStream_t s,
+                 Sums *sums = nullptr)
 {
     AVC_REQUIRE((int64_t)p.tiles_m * p.tiles_n * p.splits < (1 << 22), AVC_ERR_ARG, "avc_linear: %lld x %lld outputs are more than one launch covers", (long long)M, (long long)N);
     TileArgs a{P, Q, M, N, K, out, ldo, e, (float *)ws, p.kper, p.tiles_m, p.tiles_n, p.splits};
     const int rc = dtype == AVC_F32 ? launch_tile_f32(a, p.tile, s) : dtype == AVC_BF16 ? launch_tile_bf16(a, p.tile, s) : launch_tile_f16(a, p.tile, s);
     if (rc != AVC_OK || p.splits == 1) return rc;
-    if (dtype == AVC_F32) return launch_reduce<float>(a.partial, p.splits, M, N, out, ldo, e, s);
-    if (dtype == AVC_BF16) return launch_reduce<__bf16>(a.partial, p.splits, M, N, out, ldo, e, s);
-    return launch_reduce<_Float16>(a.partial, p.splits, M, N, out, ldo, e, s);
+    if (dtype == AVC_F32) return launch_reduce<float>(a.partial, p.splits, M, N, out, ldo, e, sums, s);
+    if (dtype == AVC_BF16) return launch_reduce<__bf16>(a.partial, p.splits, M, N, out, ldo, e, sums, s);
+    return launch_reduce<_Float16>(a.partial, p.splits, M, N, out, ldo, e, sums, s);
 }
 
 inline const void *ahead(const void *p, int64_t elements, int dtype) { return p ? (const char *)p + elements * esize(dtype) : nullptr; }
@@ -464,7 +511,7 @@ Epilogue from(const Epilogue &e, int64_t m, int64_t n, int dtype)
     return Epilogue{ahead(e.bias, n, dtype), ahead(e.res, m * e.ldr + n, dtype), e.ldr, (void *)ahead(e.z, m * e.ldz + n, dtype), e.ldz, e.act, e.slope};
 }
 
-int product(const Operand &P, const Operand &Q, int64_t M, int64_t N, int64_t K, int dtype, const Epilogue &e, void *out, int64_t ldo, void *ws, hipStream_t s)
+int product(const Operand &P, const Operand &Q, int64_t M, int64_t N, int64_t K, int dtype, const Epilogue &e, void *out, int64_t ldo, void *ws, hipStream_t s, Sums *sums = nullptr)
 {
     if (M > MOST_ROWS) {
         for (int64_t m = 0; m < M; m += MOST_ROWS) {
@@ -482,7 +529,7 @@ int product(const Operand &P, const Operand &Q, int64_t M, int64_t N, int64_t K,
         const int rc = product_part(P, from(Q, c.cols, dtype), M, N - c.cols, K, dtype, from(e, 0, c.cols, dtype), (void *)ahead(out, c.cols, dtype), ldo, ws, c.right, s);
         if (rc != AVC_OK) return rc;
     }
-    return product_part(P, Q, c.rows, c.cols, K, dtype, e, out, ldo, ws, c.main, s);
+    return product_part(P, Q, c.rows, c.cols, K, dtype, e, out, ldo, ws, c.main, s, sums);
 }
 
 // ---- few rows ----------------------------------------------------------------------------------------------------------------------------------------------------
@@ -659,15 +706,13 @@ int backward(const void *dy, int64_t lddy, const Operand &x, const void *w, int6
     char *dz_buf = (char *)ws, *strips_buf = dz_buf + sp.dz, *x_buf = strips_buf + sp.strips, *w_buf = x_buf + sp.x, *part = w_buf + sp.w;
     const bool active = act != AVC_ACT_NONE, through = active || sp.pad_dy;      // dz is dy itself, or goes through the pass below
     const int64_t lddz = through ? ceil8(N) : lddy;
+    Sums sums{};
     if (through || db) {
         const int64_t strips = strips_for(M, N, dtype);
         const int rc = AVC_BY_TYPE(dtype, launch_dact)(dy, lddy, active ? z : nullptr, ldz, act, slope, M, N, through ? dz_buf : nullptr, lddz, db && strips > 1 ? (float *)strips_buf : nullptr,
                                                        strips == 1 ? db : nullptr, strips, s);
         if (rc != AVC_OK) return rc;
-        if (db && strips > 1) {
-            const int rc2 = launch_columns((const float *)strips_buf, (int)strips, N, N, dtype, db, nullptr, s);
-            if (rc2 != AVC_OK) return rc2;
-        }
+        if (db && strips > 1) sums = Sums{(const float *)strips_buf, (int)strips, N, db};
     }
     const void *dz = through ? dz_buf : dy;
     if (dx && M) {
@@ -687,9 +732,10 @@ int backward(const void *dy, int64_t lddy, const Operand &x, const void *w, int6
             if (rc != AVC_OK) return rc;
             Q = Operand{x_buf, x.kc ? ceil8(K) : ceil8(M), x.kc ? 0 : 1, 1};
         }
-        const int rc = product(Operand{dz, lddz, 0, through}, Q, N, K, M, dtype, none, dw, K, part, s);
+        const int rc = product(Operand{dz, lddz, 0, through}, Q, N, K, M, dtype, none, dw, K, part, s, &sums);
         if (rc != AVC_OK) return rc;
     }
+    if (sums.out) return launch_columns(sums.part, sums.strips, N, N, dtype, db, nullptr, s);
     return AVC_OK;
 }
 

@@ -22,22 +22,22 @@ DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}                
 ACTS = {None: 0, 'relu': 1, 'leaky_relu': 2, 'soft_plus': 3, 'sigmoid': 4, 'tanh': 5, 'gelu': 6, 'silu': 7}   # avc_act
 
 
-def _check(who, first, **others):
-    if not isinstance(first, torch.Tensor):
-        raise TypeError(f'{who}: x: expected a torch.Tensor, got {type(first).__name__}')
-    if not first.is_cuda:
-        raise RuntimeError(f'{who} runs on the HIP device only; there is no CPU path (x lives on {first.device})')
-    if first.dtype not in DTYPES:
-        raise TypeError(f'{who}: float32, bfloat16 or float16, got {first.dtype}')
-    for name, t in others.items():
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f'{who}: {name}: expected a torch.Tensor, got {type(t).__name__}')
-        if t.dtype != first.dtype:
-            raise TypeError(f'{who}: {name} is {t.dtype}, x is {first.dtype}')
-        if t.device != first.device:
-            raise RuntimeError(f'{who}: {name} lives on {t.device}, x on {first.device}')
+def _check_first(who, x):
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f'{who}: x: expected a torch.Tensor, got {type(x).__name__}')
+    if not x.is_cuda:
+        raise RuntimeError(f'{who} runs on the HIP device only; there is no CPU path (x lives on {x.device})')
+    if x.dtype not in DTYPES:
+        raise TypeError(f'{who}: float32, bfloat16 or float16, got {x.dtype}')
+
+
+def _check_like(who, name, t, x):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f'{who}: {name}: expected a torch.Tensor, got {type(t).__name__}')
+    if t.dtype is not x.dtype:
+        raise TypeError(f'{who}: {name} is {t.dtype}, x is {x.dtype}')
+    if t.get_device() != x.get_device():
+        raise RuntimeError(f'{who}: {name} lives on {t.device}, x on {x.device}')
 
 
 _ROW_TOP, _COLUMN_TOP = 1 << 22, 1 << 25                                          # include/avcap.h: the strides that the kernels address
@@ -109,7 +109,7 @@ def _linear_forward(x, w, bias, res, act, slope, want_z):
     z = x.new_empty((m, n)) if want_z else None
     nbytes = _forward_bytes(m, n, k, dt, xr, xc)
     ws = _space(nbytes, x)
-    _lib.check(_lib.lib().avc_linear(_lib.ctx(x.device), x.data_ptr(), xr, xc, w.data_ptr(), _row_stride(w), _ptr(bias), _ptr(res), 0 if res is None else _row_stride(res), act, slope, m, n, k,
+    _lib.check(_lib.lib().avc_linear(_lib.ctx(x.get_device()), x.data_ptr(), xr, xc, w.data_ptr(), _row_stride(w), _ptr(bias), _ptr(res), 0 if res is None else _row_stride(res), act, slope, m, n, k,
                                      dt, y.data_ptr(), n, _ptr(z), n, _ptr(ws), nbytes, _stream(x)))
     return y, z
 
@@ -140,7 +140,7 @@ class _Linear(torch.autograd.Function):
             db = g.new_empty((n,)) if need_b else None
             nbytes = _backward_bytes(m, n, k, dt)
             ws = _space(nbytes, g)
-            _lib.check(_lib.lib().avc_linear_backward(_lib.ctx(g.device), g.data_ptr(), _row_stride(g), x.data_ptr(), xr, xc, w.data_ptr(), _row_stride(w), _ptr(saved), n, ctx.act, ctx.slope,
+            _lib.check(_lib.lib().avc_linear_backward(_lib.ctx(g.get_device()), g.data_ptr(), _row_stride(g), x.data_ptr(), xr, xc, w.data_ptr(), _row_stride(w), _ptr(saved), n, ctx.act, ctx.slope,
                                                       m, n, k, dt, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes, _stream(g)))
         return dx, dw, db, dy if need_r else None, None, None
 
@@ -153,7 +153,12 @@ def linear(x, weight, bias=None, act=None, slope=0.02, residual=None):
     unit stride; other layouts are copied.  Sums are float32 and each output is rounded once; float32 products keep 24 bits."""
     if act not in ACTS:
         raise ValueError(f'linear: unknown activation {act!r}, known are {[a for a in ACTS if a]}')
-    _check('linear', x, weight=weight, bias=bias, residual=residual)
+    _check_first('linear', x)
+    _check_like('linear', 'weight', weight, x)
+    if bias is not None:
+        _check_like('linear', 'bias', bias, x)
+    if residual is not None:
+        _check_like('linear', 'residual', residual, x)
     if weight.dim() == 3 and weight.shape[2] == 1:
         weight = weight[:, :, 0]
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
@@ -161,11 +166,10 @@ def linear(x, weight, bias=None, act=None, slope=0.02, residual=None):
     n, k = weight.shape
     if n < 1 or k < 1:
         raise ValueError(f'linear: a weight of shape {tuple(weight.shape)} has no values')
-    if bias is not None and tuple(bias.shape) != (n,):
+    if bias is not None and (bias.dim() != 1 or bias.shape[0] != n):
         raise ValueError(f'linear: bias {tuple(bias.shape)} for {n} outputs')
     if residual is not None and residual.shape != x.shape[:-1] + (n,):
         raise ValueError(f'linear: residual {tuple(residual.shape)}, the output is {tuple(x.shape[:-1]) + (n,)}')
-    slope = float(slope)
     if act == 'leaky_relu' and not 0.0 <= slope < float('inf'):
         raise ValueError(f'linear: leaky_relu takes a finite slope >= 0, got {slope}')
     m = x.numel() // k
@@ -187,7 +191,7 @@ def _norm_forward(x, g, b, eps, want_stats):
     y = x.new_empty((m, c))
     stats = x.new_empty((2, m), dtype=torch.float32) if want_stats else None
     p = _ptr(stats)
-    _lib.check(_lib.lib().avc_layer_norm(_lib.ctx(x.device), x.data_ptr(), _row_stride(x), _ptr(g), _ptr(b), eps, m, c, DTYPES[x.dtype], y.data_ptr(), c, p, p + 4 * m if p else p, _stream(x)))
+    _lib.check(_lib.lib().avc_layer_norm(_lib.ctx(x.get_device()), x.data_ptr(), _row_stride(x), _ptr(g), _ptr(b), eps, m, c, DTYPES[x.dtype], y.data_ptr(), c, p, p + 4 * m if p else p, _stream(x)))
     return y, stats
 
 
@@ -211,25 +215,30 @@ class _LayerNorm(torch.autograd.Function):
         nbytes = _norm_backward_bytes(m, c, dt) if need_g or need_b else 0
         ws = _space(nbytes, dy)
         p = stats.data_ptr()
-        _lib.check(_lib.lib().avc_layer_norm_backward(_lib.ctx(dy.device), dy.data_ptr(), _row_stride(dy), x.data_ptr(), _row_stride(x), _ptr(g), p, p + 4 * m, m, c, dt, _ptr(dx), c, _ptr(dg),
+        _lib.check(_lib.lib().avc_layer_norm_backward(_lib.ctx(dy.get_device()), dy.data_ptr(), _row_stride(dy), x.data_ptr(), _row_stride(x), _ptr(g), p, p + 4 * m, m, c, dt, _ptr(dx), c, _ptr(dg),
                                                       _ptr(db), _ptr(ws), nbytes, _stream(dy)))
         return dx, dg, db, None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """The layer norm over the last axis: x (..., C), weight and bias (C) or None -> (..., C).  Mean and biased variance in float32, the variance from centred values."""
-    _check('layer_norm', x, weight=weight, bias=bias)
+    _check_first('layer_norm', x)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f'layer_norm: x {tuple(x.shape)} has no values along its last axis')
     c = x.shape[-1]
     for name, t in (('weight', weight), ('bias', bias)):
-        if t is not None and tuple(t.shape) != (c,):
-            raise ValueError(f'layer_norm: {name} {tuple(t.shape)} for rows of {c}')
+        if t is not None:
+            _check_like('layer_norm', name, t, x)
+            if t.dim() != 1 or t.shape[0] != c:
+                raise ValueError(f'layer_norm: {name} {tuple(t.shape)} for rows of {c}')
     eps = float(eps)
     if not 0.0 <= eps < float('inf'):
         raise ValueError(f'layer_norm: eps must be finite and >= 0, got {eps}')
     x2 = x if x.dim() == 2 else x.reshape(x.numel() // c, c)
-    weight, bias = (t if t is None or c == 1 or t.stride(0) == 1 else t.contiguous() for t in (weight, bias))
+    if weight is not None and weight.stride(0) != 1:
+        weight = weight.contiguous()
+    if bias is not None and bias.stride(0) != 1:
+        bias = bias.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
         y = _LayerNorm.apply(x2, weight, bias, eps)
     else:
