@@ -62,7 +62,13 @@ template <int BR, bool KC> struct Tile {
     static constexpr int BYTES = ROWS * ROW_BYTES;
     __device__ static __forceinline__ int swizzle(int row)
     {
-        if constexpr (KC) return BK == 64 ? (row >> 1) & 7 : (row >> 2) & 3;
+        if constexpr (KC) {
+            if (BK == 64) return (row >> 1) & 7;
+            // 64-byte rows: a 16-byte read is served 16 lanes at a time, rows 0 - 3 and 12 - 15 of one quarter with rows 4 - 11 of the next, so four groups of four rows at two
+            // pieces have to differ: 0 2 3 1 by group (0 1 2 3 met itself: 39 % of the LDS cycles were conflicts)
+            const int g = (row >> 2) & 3, x = g ^ (g >> 1);
+            return ((x & 1) << 1) | (x >> 1);
+        }
         else return (((row & 3) | (((row >> 3) & 1) << 2)) << 1) & (PIECES - 1);
     }
     // byte of piece p of row `row`
