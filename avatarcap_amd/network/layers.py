@@ -6,7 +6,7 @@
 `linear` is what one step of the reference's `MLP.forward` does (network/mlp.py:56-72: a Conv1d(k=1) and its activation), for any widths; network/mlp.py calls it.  Tensors are
 float32, bfloat16 or float16, all of one call alike, on the HIP device; there is no CPU path.  Both run on the current stream of the tensors' device, whichever device is current,
 take their workspace from torch's allocator (so a captured graph keeps its own) and have a backward pass of the same kernels (csrc/linear.hip, linear_tile.hip, layer_norm.hip).
-No gradient of a gradient.
+No gradient of a gradient: taking one raises.
 """
 from __future__ import annotations
 
@@ -14,7 +14,6 @@ import ctypes as C
 import functools
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 
@@ -99,6 +98,27 @@ def _stream(t):
     return torch._C._cuda_getCurrentRawStream(t.get_device())         # what torch.cuda.current_stream(t.device).cuda_stream is, without the objects around it
 
 
+class _NoSecond(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, live, *grads):
+        return tuple(g.detach() for g in grads)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError('linear, layer_norm: the gradients have no derivative of their own')
+
+
+def _once(backward, ctx, dy):
+    """The backward pass under create_graph, which is when the engine leaves gradients enabled: a derivative taken of its results raises, whether dy itself carries a graph or not,
+    instead of leaving out what runs through x and the weights."""
+    with torch.no_grad():
+        out = list(backward(ctx, dy))
+    at = [i for i, g in enumerate(out) if g is not None and g is not dy]
+    for i, g in zip(at, _NoSecond.apply(torch.zeros((), requires_grad=True), *[out[i] for i in at]) if at else ()):
+        out[i] = g
+    return tuple(out)
+
+
 def _linear_forward(x, w, bias, res, act, slope, want_z):
     m, k = x.shape
     n = w.shape[0]
@@ -114,6 +134,25 @@ def _linear_forward(x, w, bias, res, act, slope, want_z):
     return y, z
 
 
+def _linear_backward(ctx, dy):
+    x, w, saved = ctx.saved_tensors
+    need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+    dx = dw = db = None
+    if need_x or need_w or need_b:
+        (m, k), n, dt = x.shape, w.shape[0], DTYPES[dy.dtype]
+        g = _rows(dy)
+        x, xr, xc = _matrix(x, _ROW_TOP)
+        w = _rows(w)
+        dx = g.new_empty((m, k)) if need_x else None
+        dw = g.new_empty((n, k)) if need_w else None
+        db = g.new_empty((n,)) if need_b else None
+        nbytes = _backward_bytes(m, n, k, dt)
+        ws = _space(nbytes, g)
+        _lib.check(_lib.lib().avc_linear_backward(_lib.ctx(g.get_device()), g.data_ptr(), _row_stride(g), x.data_ptr(), xr, xc, w.data_ptr(), _row_stride(w), _ptr(saved), n, ctx.act, ctx.slope,
+                                                  m, n, k, dt, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes, _stream(g)))
+    return dx, dw, db, dy if need_r else None, None, None
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, res, act, slope):
@@ -125,24 +164,8 @@ class _Linear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, w, saved = ctx.saved_tensors
-        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        dx = dw = db = None
-        if need_x or need_w or need_b:
-            (m, k), n, dt = x.shape, w.shape[0], DTYPES[dy.dtype]
-            g = _rows(dy)
-            x, xr, xc = _matrix(x, _ROW_TOP)
-            w = _rows(w)
-            dx = g.new_empty((m, k)) if need_x else None
-            dw = g.new_empty((n, k)) if need_w else None
-            db = g.new_empty((n,)) if need_b else None
-            nbytes = _backward_bytes(m, n, k, dt)
-            ws = _space(nbytes, g)
-            _lib.check(_lib.lib().avc_linear_backward(_lib.ctx(g.get_device()), g.data_ptr(), _row_stride(g), x.data_ptr(), xr, xc, w.data_ptr(), _row_stride(w), _ptr(saved), n, ctx.act, ctx.slope,
-                                                      m, n, k, dt, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes, _stream(g)))
-        return dx, dw, db, dy if need_r else None, None, None
+        return _once(_linear_backward, ctx, dy) if torch.is_grad_enabled() else _linear_backward(ctx, dy)
 
 
 def linear(x, weight, bias=None, act=None, slope=0.02, residual=None):
@@ -195,6 +218,22 @@ def _norm_forward(x, g, b, eps, want_stats):
     return y, stats
 
 
+def _norm_backward(ctx, dy):
+    x, g, stats = ctx.saved_tensors
+    need_x, need_g, need_b = ctx.needs_input_grad[:3]
+    (m, c), dt = x.shape, DTYPES[dy.dtype]
+    x, dy = _rows(x), _rows(dy)
+    dx = dy.new_empty((m, c)) if need_x else None
+    dg = dy.new_empty((c,)) if need_g else None
+    db = dy.new_empty((c,)) if need_b else None
+    nbytes = _norm_backward_bytes(m, c, dt) if need_g or need_b else 0
+    ws = _space(nbytes, dy)
+    p = stats.data_ptr()
+    _lib.check(_lib.lib().avc_layer_norm_backward(_lib.ctx(dy.get_device()), dy.data_ptr(), _row_stride(dy), x.data_ptr(), _row_stride(x), _ptr(g), p, p + 4 * m, m, c, dt, _ptr(dx), c, _ptr(dg),
+                                                  _ptr(db), _ptr(ws), nbytes, _stream(dy)))
+    return dx, dg, db, None
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, g, b, eps):
@@ -203,21 +242,8 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, g, stats = ctx.saved_tensors
-        need_x, need_g, need_b = ctx.needs_input_grad[:3]
-        (m, c), dt = x.shape, DTYPES[dy.dtype]
-        x, dy = _rows(x), _rows(dy)
-        dx = dy.new_empty((m, c)) if need_x else None
-        dg = dy.new_empty((c,)) if need_g else None
-        db = dy.new_empty((c,)) if need_b else None
-        nbytes = _norm_backward_bytes(m, c, dt) if need_g or need_b else 0
-        ws = _space(nbytes, dy)
-        p = stats.data_ptr()
-        _lib.check(_lib.lib().avc_layer_norm_backward(_lib.ctx(dy.get_device()), dy.data_ptr(), _row_stride(dy), x.data_ptr(), _row_stride(x), _ptr(g), p, p + 4 * m, m, c, dt, _ptr(dx), c, _ptr(dg),
-                                                      _ptr(db), _ptr(ws), nbytes, _stream(dy)))
-        return dx, dg, db, None
+        return _once(_norm_backward, ctx, dy) if torch.is_grad_enabled() else _norm_backward(ctx, dy)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):

@@ -372,6 +372,22 @@ def test_shapes_views_and_partial_gradients():
         d.sum().backward()
 
 
+@pytest.mark.parametrize('what', ['linear', 'bias only', 'layer_norm'])
+@pytest.mark.parametrize('graph_in_dy', [False, True])
+def test_a_derivative_of_the_gradients_raises_and_leaves_nothing_out(what, graph_in_dy):
+    q = torch.randn(4, 24, device='cuda', requires_grad=what != 'bias only')
+    b = torch.randn(24, device='cuda', requires_grad=True)
+    w = torch.randn(24, 24, device='cuda')
+    y = layer_norm(q, b) if what == 'layer_norm' else linear(q, w, b, act='tanh', residual=q)
+    dy = torch.ones(4, 24, device='cuda', requires_grad=graph_in_dy)
+    leaf = b if what == 'bias only' else q
+    (plain,) = torch.autograd.grad(y, leaf, dy.detach(), retain_graph=True)
+    (d,) = torch.autograd.grad(y, leaf, dy, create_graph=True)
+    assert torch.equal(d.detach(), plain)
+    with pytest.raises(RuntimeError, match='no derivative'):
+        (d.sum() + y.sum()).backward()                                      # y's own part would go through: the sum must not
+
+
 @pytest.mark.parametrize('dtype', DTYPES)
 def test_the_same_bits_every_time_and_on_another_stream(dtype):
     xd, x, w, b, r, dy = make(3000, 264, 200, dtype, residual=True)
