@@ -12,7 +12,7 @@ namespace {
 template <typename T> __device__ __forceinline__ void finish(float v, int64_t m, int64_t n, const Epilogue &e, T *out, int64_t ldo)
 {
     if (e.bias) v += (float)((const T *)e.bias)[n];
-    if (e.z) ((T *)e.z)[m * e.ldz + n] = (T)v;
+    if (e.z) ((T *)e.z)[m * e.ldz + n] = keep_z<T>(v, e.act);
     float a[1] = {v};
     act_run<sizeof(T) == 2, 1>(a, e.act, e.slope);
     v = a[0];
@@ -133,7 +133,7 @@ template <typename T, int FB> __global__ __launch_bounds__(1024) void few_kernel
         const bool mine = 16 * b + l16 < a.nf;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (a.ep.z && mine && s0 + 4 * q + j < a.ns) ((T *)a.ep.z)[m[j] * a.ep.ldz + n[j]] = (T)v[j];
+            if (a.ep.z && mine && s0 + 4 * q + j < a.ns) ((T *)a.ep.z)[m[j] * a.ep.ldz + n[j]] = keep_z<T>(v[j], a.ep.act);
         act_run<sizeof(T) == 2, 4>(v, a.ep.act, a.ep.slope);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -248,8 +248,7 @@ template <typename T, bool SHORT> __global__ __launch_bounds__(256) void dact_ke
             if (z) {
                 const vec s = read_run<T, SHORT>(z + m * ldz, n, N);
                 float zs[V], sl[V];
-#pragma unroll
-                for (int j = 0; j < V; ++j) zs[j] = (float)s[j];
+                kept_z<T, V>(s, zs, act);
                 slope_run<sizeof(T) == 2, V>(zs, sl, act, slope);
 #pragma unroll
                 for (int j = 0; j < V; ++j) v[j] *= sl[j];
@@ -356,7 +355,7 @@ template <typename T> __global__ __launch_bounds__(1024) void reduce_kernel(cons
         vec o;
         if (e.z) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] = (T)v[j];
+            for (int j = 0; j < 4; ++j) o[j] = keep_z<T>(v[j], e.act);
             *reinterpret_cast<loose *>((T *)e.z + m * e.ldz + n) = o;
         }
         act_run<sizeof(T) == 2, 4>(v, e.act, e.slope);

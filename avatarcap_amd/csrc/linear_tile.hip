@@ -287,8 +287,7 @@ template <int BR, bool KC, int NT> struct StagedSlope {
             elem8 x = g.v[i];
             if (act != AVC_ACT_NONE) {
                 float zs[8], sl[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) zs[j] = (float)z.v[i][j];
+                kept_z<elem_t, 8>(z.v[i], zs, act);
                 slope_run<!IS_F32, 8>(zs, sl, act, slope);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] = (elem_t)((float)x[j] * sl[j]);
@@ -355,13 +354,13 @@ template <int READS, int MFMAS, int LOADS> __device__ __forceinline__ void inter
 }
 
 // 16 bytes of a row, of any alignment; what passes the row's end is left out.  (One store of a vector type: of a copy from an array the compiler makes several.)
-template <int VEC> __device__ __forceinline__ void store_run(elem_t *dst, const float *v, int64_t left)
+template <int VEC, typename T> __device__ __forceinline__ void store_run(T *dst, const float *v, int64_t left)
 {
-    typedef elem_t vec __attribute__((ext_vector_type(VEC)));
-    typedef vec loose __attribute__((aligned(sizeof(elem_t))));
+    typedef T vec __attribute__((ext_vector_type(VEC)));
+    typedef vec loose __attribute__((aligned(sizeof(T))));
     vec o;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) o[j] = (elem_t)v[j];
+    for (int j = 0; j < VEC; ++j) o[j] = (T)v[j];
     if (left >= VEC) *reinterpret_cast<loose *>(dst) = o;
     else
 #pragma unroll
@@ -555,7 +554,10 @@ __device__ __forceinline__ void tile_body(const TileArgs &a, const Slope &dz, un
                 for (int k = 0; k < 4; ++k) v[j + k] = x[k] + bias[j + k];
             }
             if (m >= a.M || left <= 0) continue;
-            if (e.z) store_run<VEC>((elem_t *)e.z + m * e.ldz + n, v, left);
+            if (e.z) {
+                if (KeptZ<elem_t>::finer(e.act)) store_run<VEC>((_Float16 *)e.z + m * e.ldz + n, v, left);
+                else store_run<VEC>((elem_t *)e.z + m * e.ldz + n, v, left);
+            }
             act_run<!IS_F32, VEC>(v, e.act, e.slope);
             if (e.res)
 #pragma unroll
@@ -591,12 +593,14 @@ template <bool XKC> __global__ __launch_bounds__(256, 2) void small_backward_ker
         float s = 0.f;
         for (int64_t m = ly; m < a.M; m += 16 * 4) {
             float g[4], zs[4], sl[4];
+            elem_t kept[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int64_t r = min(m + 16 * j, a.M - 1);
                 g[j] = (float)dy[r * a.lddy];
-                zs[j] = a.act != AVC_ACT_NONE ? (float)z[r * a.ld_saved] : 0.f;
+                kept[j] = a.act != AVC_ACT_NONE ? z[r * a.ld_saved] : (elem_t)0.f;
             }
+            kept_z<elem_t, 4>(kept, zs, a.act);
             slope_run<!IS_F32, 4>(zs, sl, a.act, a.slope);
 #pragma unroll
             for (int j = 0; j < 4; ++j) s += m + 16 * j < a.M ? g[j] * sl[j] : 0.f;

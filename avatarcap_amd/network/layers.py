@@ -126,7 +126,7 @@ def _linear_forward(x, w, bias, res, act, slope, want_z):
     x, xr, xc = _matrix(x)
     w = _rows(w)
     y = x.new_empty((m, n))
-    z = x.new_empty((m, n)) if want_z else None
+    z = x.new_empty((m, n)) if want_z else None            # bf16 of soft_plus ... silu: float16 bits (csrc/linear.h KeptZ)
     nbytes = _forward_bytes(m, n, k, dt, xr, xc)
     ws = _space(nbytes, x)
     _lib.check(_lib.lib().avc_linear(_lib.ctx(x.get_device()), x.data_ptr(), xr, xc, w.data_ptr(), _row_stride(w), _ptr(bias), _ptr(res), 0 if res is None else _row_stride(res), act, slope, m, n, k,

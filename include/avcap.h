@@ -163,7 +163,8 @@ enum avc_act { AVC_ACT_NONE = 0, AVC_ACT_RELU = 1, AVC_ACT_LEAKY_RELU = 2 /* z >
 /* z = x w^T + bias, y = act(z) + res.
  *   x (M, K) at x[m * x_row + k * x_col], one of the two strides being 1 (x_col = 1: rows of points; x_row = 1: channel-first points as Conv1d has them)
  *   w (N, K) rows of K adjacent values, ldw apart;  bias (N) or NULL;  res (M, N), ldr apart, or NULL
- *   y (M, N), ldy apart;  z (M, N), ldz apart, or NULL: the value before the activation, which the backward pass reads.  y, z overlap no input (y may be res itself).
+ *   y (M, N), ldy apart;  z (M, N), ldz apart, or NULL: the value before the activation, which the backward pass reads (in bf16 calls float16 from AVC_ACT_SOFTPLUS on).  y, z overlap no
+ *   input (y may be res itself).
  * M >= 0, N, K >= 1.  A NaN or infinity of x or w reaches exactly the outputs it has a part in.
  * Row strides (of x with x_col = 1, w, dy, saved) below 2^22 elements; x_col of channel-first points below 2^25 here, below 2^22 in the backward pass (AVC_ERR_ARG beyond). */
 int avc_linear_workspace(int64_t M, int64_t N, int64_t K, int dtype, int64_t x_row, int64_t x_col, int64_t *bytes);
